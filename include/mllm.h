@@ -44,6 +44,14 @@ extern "C" {
 #define MLLM_ERR_UNSUPPORTED 4 /* shape/format this build does not handle */
 #define MLLM_ERR_DEVICE 5      /* a kernel reported an error (e.g. barrier time-out) */
 
+/* Storage codes: the PGW1 dtype codes (weights.js:3) plus 5 = Q8 group-32. */
+#define MLLM_F32 0
+#define MLLM_F16 1
+#define MLLM_BF16 2
+#define MLLM_Q8 3
+#define MLLM_Q4 4
+#define MLLM_Q8G32 5
+
 /* Thread-local message for the last non-zero return (never NULL). */
 const char *mllm_last_error(void);
 
@@ -121,6 +129,95 @@ int mllm_silu_mul(int n, float *a, const float *b, void *stream);
 /* weights.js:106-123 dequantizeToF32 (q4 branch): out[m][n], bit-exact. */
 int mllm_dequant_q4(int m, int n, const uint8_t *packed, const float *scale, int group, float *out, void *stream);
 
+/* ------------------------------------------------------------------------
+ * A decode step of several sequences (no counterpart in the reference, whose
+ * engine holds one sequence): with mllm_rms_norm, mllm_gemm_q4 and
+ * mllm_silu_mul around them, the next three operators are the step's
+ * attention -- mllm_rope_kv_paged (infer.js:422-460 for one sequence),
+ * mllm_attn_paged (infer.js:461-504) -- and its choice of tokens, mllm_sample.
+ * They allocate nothing and keep nothing between calls, so they may be
+ * captured into a graph, and calls on different streams may overlap.
+ * ------------------------------------------------------------------------ */
+
+/* A pool of key-value pages and the page table of the sequences in it.
+ * Element d of KV head h of a slot lies at
+ *   page * page_stride + h * head_stride + slot * row_stride + d
+ * of k and of v; three zero strides mean [pages][n_kv_heads][page_size][head_dim].
+ * Position p of sequence s is slot p % page_size of page table[s][p / page_size].
+ * Sequences may share pages.  k, v and the strides are 16-byte aligned. */
+typedef struct mllm_kv_pages {
+  void *k, *v;
+  int32_t storage; /* MLLM_F32, MLLM_F16 or MLLM_BF16 */
+  int32_t n_kv_heads, head_dim; /* head_dim a multiple of 32, at most 256 */
+  int32_t pages, page_size;     /* any page_size >= 1 */
+  int64_t page_stride, head_stride, row_stride; /* in elements */
+  const int32_t *table; /* device [sequences][table_cols] */
+  int32_t sequences, table_cols;
+} mllm_kv_pages;
+
+/* The rows of attn.qkv into rotated queries and the cache.  qkv is
+ * [tokens][(n_heads + 2 n_kv_heads) head_dim], queries, keys, values; token t
+ * stands at position pos[t] of sequence seq[t] (seq NULL: sequence t).
+ *   - q_gain / k_gain (head_dim values, NULL: no norm): each head of the
+ *     queries / keys times gain / sqrt(mean of its squares + eps) first.
+ *   - Elements 0 .. rot - 1 of each query and key head are rotated, the others
+ *     pass through: pairs (i, i + rot / 2) (applyRope, infer.js:208-225), or
+ *     (2i, 2i + 1) where interleaved != 0, by the angle pos * inv_freq[i],
+ *     i < rot / 2, formed in double.  A context scaled for more positions is a
+ *     matter of inv_freq.  rot = 0 rotates nothing (inv_freq may be NULL).
+ *   - q receives [tokens][n_heads head_dim]; keys and values go to the token's
+ *     slot, rounded to nearest even (f16: beyond 65504 to infinity).
+ * A token whose sequence is outside [0, sequences), or whose position is
+ * negative, is padding: nothing is written for it.  One whose position has no
+ * page -- beyond the table, or the table's entry outside [0, pages) -- writes q
+ * alone.  Two tokens of one call must not share a slot. */
+int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const float *qkv, const int32_t *seq,
+                       const int32_t *pos, const float *inv_freq, int rot, int interleaved, const float *q_gain,
+                       const float *k_gain, float eps, float *q, void *stream);
+
+/* out[r] = softmax(scale q[r] K^T) V for rows of one token: q and out are
+ * [rows][n_heads head_dim], query head h reads KV head h n_kv_heads / n_heads
+ * (n_heads a multiple of n_kv_heads), and row r attends to positions 0 ..
+ * len[r] - 1 of sequence seq[r] (seq NULL: sequence r).  Several rows may have
+ * one sequence: a speculation pass is a row per token, each one longer.
+ * max_len bounds every len (at most page_size * table_cols); the work is split
+ * over it, so a host passes the longest it knows of.
+ *   - len[r] = 0: out[r] is 0.  A sequence outside [0, sequences) is padding:
+ *     out[r] is left as it was.
+ *   - len[r] < 0 or > max_len, or a page within the length outside [0, pages):
+ *     out[r] (the heads' rows) is NaN.
+ *   - Only positions below len[r] count, whatever the slots behind them hold.
+ *     Infinities and NaN within it act as in infer.js:461-504.
+ * All products and sums are float32.  The workspace is
+ * mllm_attn_paged_workspace() bytes, 16-byte aligned, of any contents (NULL
+ * where that is 0); calls that may overlap need one each. */
+int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, const float *q, const int32_t *seq,
+                    const int32_t *len, int max_len, float scale, float *out, void *workspace,
+                    uint64_t workspace_bytes, void *stream);
+/* Its bytes for these arguments (0 also for arguments that the call refuses). */
+uint64_t mllm_attn_paged_workspace(const mllm_kv_pages *kv, int rows, int n_heads, int max_len);
+
+/* ids[r]: a token drawn from each row of logits [rows][vocab] with the random
+ * number u[r] of [0, 1); probs[r] (nullable) its probability among the tokens
+ * that were left.  Each row has its own settings (device arrays, NULL: off):
+ *   weights w_i = exp((logit_i - max) / temperature) (NULL: temperature 1);
+ *   the tokens in order: larger logit first, equal ones by index;
+ *   top_k > 0 keeps the first top_k of them; then
+ *   top_p < 1 the shortest prefix whose weights reach top_p of what is left; then
+ *   min_p > 0 those of weight >= min_p; the first token stays in any case;
+ * and the draw takes the first token, by index, at which the running sum of
+ * the weights left passes u times their total.
+ *   - temperature <= 0 (or NaN): the first maximum (argmax, infer.js:240-250),
+ *     probability 1.
+ *   - NaN and -inf have no weight.  A row without any other value: id 0,
+ *     probability 0.  +inf: only the tokens at +inf have weight.
+ *   - u below 0 or NaN counts as 0, u >= 1 as the last token left.
+ * Weights are whole numbers of 2^-44 of the largest, so the sums are exact and
+ * a row draws the same token in any batch; weights below 2^-44 count as 0.
+ * vocab is at most 524288. */
+int mllm_sample(int rows, int vocab, const float *logits, const float *temperature, const int32_t *top_k,
+                const float *top_p, const float *min_p, const float *u, int32_t *ids, float *probs, void *stream);
+
 /* ========================================================================
  * Engine level (infer.js PetitGPT)
  * ====================================================================== */
@@ -134,14 +231,6 @@ typedef struct mllm_config {
   float norm_eps;  /* RMSNorm eps; the reference uses 1e-6 (infer.js:8) */
   int32_t kv_fp16; /* 0: f32 KV cache as the reference; 1: fp16 KV cache */
 } mllm_config;
-
-/* Storage codes: the PGW1 dtype codes (weights.js:3) plus 5 = Q8 group-32. */
-#define MLLM_F32 0
-#define MLLM_F16 1
-#define MLLM_BF16 2
-#define MLLM_Q8 3
-#define MLLM_Q4 4
-#define MLLM_Q8G32 5
 
 /* One entry of the PGW1 JSON tensor table (convert_hf_to_pgw.py:44-69);
  * offsets are relative to the payload start. */

@@ -17,9 +17,19 @@ LIB_PATH = os.environ.get("MLLM_LIBRARY") or os.path.join(PKG_DIR, "libmllm.so")
 MLLM_OK = 0
 ERR_NAMES = {1: "INVALID", 2: "HIP", 3: "OOM", 4: "UNSUPPORTED", 5: "DEVICE"}
 
+class MllmKvPages(C.Structure):
+    """mllm_kv_pages (include/mllm.h): pointers are device addresses."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("storage", C.c_int32), ("n_kv_heads", C.c_int32),
+                ("head_dim", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32),
+                ("page_stride", C.c_int64), ("head_stride", C.c_int64), ("row_stride", C.c_int64),
+                ("table", C.c_void_p), ("sequences", C.c_int32), ("table_cols", C.c_int32)]
+
+
 # Every exported entry point with its argument and return types.
 P = C.c_void_p
 I = C.c_int
+F = C.c_float
+KV = C.POINTER(MllmKvPages)  # an MllmKvPages is passed as it is
 SIGNATURES = {
     "mllm_last_error": ([], C.c_char_p),
     "mllm_kernel_version": ([], I),
@@ -35,6 +45,10 @@ SIGNATURES = {
     "mllm_rms_norm": ([I, P, P, P, I, C.c_float, P], I),
     "mllm_silu_mul": ([I, P, P, P], I),
     "mllm_dequant_q4": ([I, I, P, P, I, P, P], I),
+    "mllm_rope_kv_paged": ([KV, I, I, P, P, P, P, I, I, P, P, F, P, P], I),
+    "mllm_attn_paged_workspace": ([KV, I, I, I], C.c_uint64),
+    "mllm_attn_paged": ([KV, I, I, P, P, P, I, F, P, P, C.c_uint64, P], I),
+    "mllm_sample": ([I, I, P, P, P, P, P, P, P, P, P], I),
     "mllm_model_create": ([P, P, C.c_uint64, P, I, P], I),
     "mllm_model_destroy": ([P], I),
     "mllm_reset_cache": ([P], I),
