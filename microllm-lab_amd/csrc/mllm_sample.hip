@@ -11,7 +11,7 @@ using namespace mllm;
 namespace {
 
 // One workgroup per row.  With d = max - z, a token's weight is
-//   W = round(2^44 2^(-d log2(e) / T)),  0 below 2^0 (d > dlim),
+//   W = round(2^44 2^(-d log2(e) / T)),  0 past 2^-44 of the largest,
 // an integer, so that every sum is exact and the same in any order: the
 // weights of up to 2^19 tokens fit 64 bits, and 2^-45 of the largest is a
 // thousandth of what float64 sums of float64 weights would need to name
@@ -20,16 +20,19 @@ namespace {
 // The order of the tokens is: larger logit first, equal ones by index.  top-k
 // and top-p both keep a prefix of it -- the shortest whose count reaches k, or
 // whose weight reaches top_p of the total -- and so does min-p.  No sort: the
-// last token of a prefix is found by histograms (count or weight per bin, in
-// LDS), each level taking the bin in which the sum passes its target: first
-// 2048 bins of equal width in d, then of equal width in the bits of the logit,
-// at most three times, and tokens that still tie by index.
+// tokens' counts or weights are summed into 2048 bins of equal width in d (LDS
+// atomics on 64-bit integers), the bin in which the running sum passes its
+// target is gathered, and each of its tokens counts what stands before it.  A
+// bin of more than 128 tokens (ties, a wide spread of logits) is split further
+// by the bits of the logit, at most three times, and then by index.
 //
 // The draw itself sums the kept weights by 256-token chunks in index order and
 // takes the first token whose running sum is more than u of the total.
 constexpr int ST = 1024;        // threads
 constexpr int SW = ST / 64;     // waves
 constexpr int SB = 2048;        // bins of a histogram, and chunks of a row at most
+constexpr int SG = 128;         // tokens of a bin that are ranked against each other
+constexpr int SL = 2048;        // tokens that fit the list of those that can be left
 constexpr int kMaxVocab = SB * 256;
 constexpr int WBITS = 44;
 
@@ -48,45 +51,82 @@ __device__ __forceinline__ uint32_t key_of(float z) {
   const uint32_t b = __float_as_uint(z + 0.0f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float of_key(uint32_t k) {
+  return __uint_as_float(k & 0x80000000u ? k ^ 0x80000000u : ~k);
+}
+
+// Values that are the same in every thread, for the scalar registers.
+__device__ __forceinline__ float uni(float v) { return readlane_f(v, 0); }
+__device__ __forceinline__ int uni(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ u64 uni(u64 v) {
+  return (u64)(uint32_t)uni((int)(uint32_t)(v >> 32)) << 32 | (uint32_t)uni((int)(uint32_t)v);
+}
+__device__ __forceinline__ double uni(double v) { return __longlong_as_double((long long)uni((u64)__double_as_longlong(v))); }
 
 // A row's state, the same in every thread.
 struct Row {
-  float zmax, dlim;
-  double c;           // log2(e) / T
-  uint32_t key_cut;   // kept: key > key_cut, or key == key_cut and index <= idx_cut
-  int idx_cut;
-  u64 wmin;           // kept: weight at least this
-  int first;          // the first token of the order, always kept
+  float zmax, slack;  // slack: more than two roundings of max - d
+  float s0;           // bins per unit of d
+  double dmax, c;     // zmax; log2(e) / T
+  float zcut;         // kept: z > zcut, or z == zcut and index <= icut (never NaN or -inf)
+  int icut;
 };
 
-__device__ __forceinline__ float dist(const Row &R, float z) { return z == R.zmax ? 0.f : R.zmax - z; }
-__device__ __forceinline__ bool live(const Row &R, float z) { return dist(R, z) <= R.dlim; }  // not NaN, not -inf
+__device__ __forceinline__ bool kept(const Row &R, float z, int i) {
+  return z > R.zcut || (z == R.zcut && i <= R.icut);
+}
+__device__ __forceinline__ int bin_of(const Row &R, float z) { return (int)fminf((R.zmax - z) * R.s0, (float)(SB - 1)); }
+// Logits below this cannot be in bins up to b, nor those above hi_of(b) in bin b.
+__device__ __forceinline__ float lo_of(const Row &R, int b) {
+  return b >= SB - 1 || R.zmax == INFINITY ? -INFINITY : R.zmax - (float)(b + 2) / R.s0 - R.slack;
+}
+__device__ __forceinline__ float hi_of(const Row &R, int b) {
+  return b <= 1 || R.zmax == INFINITY ? R.zmax : R.zmax - (float)(b - 1) / R.s0 + R.slack;
+}
 
-// W of a live token: 2^t by its Taylor series about the nearest integer, whose
-// next term is below 2^-47, and the scaling in the exponent.
+// W of a kept token: 2^t by a polynomial in the distance to the nearest
+// integer (interpolated at Chebyshev nodes, within 8e-16; 1 at 0), the integer
+// in the exponent.
 __device__ __forceinline__ u64 weight(const Row &R, float z) {
-  const double d = z == R.zmax ? 0.0 : (double)R.zmax - (double)z, t = -d * R.c, n = rint(t), f = t - n;
-  double p = 4.4455382718708116e-10;                       // ln2^k / k!, k = 11
-  p = __builtin_fma(p, f, 7.0549116208011233e-09);
-  p = __builtin_fma(p, f, 1.0178086009239700e-07);
-  p = __builtin_fma(p, f, 1.3215486790144309e-06);
-  p = __builtin_fma(p, f, 1.5252733804059840e-05);
-  p = __builtin_fma(p, f, 1.5403530393381609e-04);
-  p = __builtin_fma(p, f, 1.3333558146428443e-03);
-  p = __builtin_fma(p, f, 9.6181291076284772e-03);
-  p = __builtin_fma(p, f, 5.5504108664821580e-02);
-  p = __builtin_fma(p, f, 2.4022650695910072e-01);
-  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+  const double t = z == R.zmax ? 0.0 : ((double)z - R.dmax) * R.c, n = rint(t), f = t - n;
+  double p = 7.070977866508139e-09;
+  p = __builtin_fma(p, f, 1.0205905413765595e-07);
+  p = __builtin_fma(p, f, 1.3215451633221434e-06);
+  p = __builtin_fma(p, f, 1.5252672924850737e-05);
+  p = __builtin_fma(p, f, 1.5403530424776529e-04);
+  p = __builtin_fma(p, f, 1.3333558200794592e-03);
+  p = __builtin_fma(p, f, 9.6181291076186650e-03);
+  p = __builtin_fma(p, f, 5.5504108664651670e-02);
+  p = __builtin_fma(p, f, 2.4022650695910075e-01);
+  p = __builtin_fma(p, f, 6.9314718055994620e-01);
   p = __builtin_fma(p, f, 1.0);
-  const long long e = (long long)__double_as_longlong(p) + ((long long)((int)n + WBITS) << 52);
-  return (u64)__double_as_longlong(__longlong_as_double(e) + 4503599627370496.0) & 0xfffffffffffffull;
+  const double w = __builtin_ldexp(p, (int)n + WBITS) + 4503599627370496.0;  // 2^52: the integer in the mantissa
+  return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
 }
 
-__device__ __forceinline__ bool in_cut(const Row &R, float z, int i) {
-  const uint32_t k = key_of(z);
-  return live(R, z) && (k > R.key_cut || (k == R.key_cut && i <= R.idx_cut));
+template <int CTRL>
+__device__ __forceinline__ u64 dpp64(u64 v) {
+  const uint32_t lo = (uint32_t)dpp_i<CTRL>((int)(uint32_t)v), hi = (uint32_t)dpp_i<CTRL>((int)(uint32_t)(v >> 32));
+  return (u64)hi << 32 | lo;
 }
-
+__device__ __forceinline__ u64 lane64(u64 v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane),
+                 hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return (u64)hi << 32 | lo;
+}
+__device__ __forceinline__ u64 sum8_64(u64 v) {  // over the 8 lanes of each half-row
+  v += dpp64<0xB1>(v);
+  v += dpp64<0x4E>(v);
+  return v + dpp64<0x141>(v);
+}
+__device__ __forceinline__ u64 sum16_64(u64 v) {  // over each row of 16
+  v = sum8_64(v);
+  return v + dpp64<0x140>(v);
+}
+__device__ __forceinline__ u64 wave_sum64(u64 v) {
+  v = sum16_64(v);
+  return (lane64(v, 0) + lane64(v, 16)) + (lane64(v, 32) + lane64(v, 48));
+}
 __device__ __forceinline__ u64 wave_incl(u64 v) {  // inclusive scan over the lanes
   const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -100,249 +140,344 @@ __device__ __forceinline__ u64 wave_incl(u64 v) {  // inclusive scan over the la
 struct Lds {
   u64 bin[SB];
   u64 wave[SW];
-  uint32_t wk[2 * SW];
   // the bin that scan_find has found: its number, the sum before it, its own sum
   int at;
   u64 before, own;
+  // the tokens that can be left
+  float lz[SL];
+  int li[SL];
+  int ln;
+  // the tokens of a bin
+  u64 gw[SG];
+  float gz[SG];
+  int gi[SG];
+  int n;
+  float zcut;
+  int icut;
   float wv[SW];
-  int wi[SW];
   int id;
 };
 
-// The first bin at which the running sum reaches target (>= 1), in L.at /
-// before / own; the total (all bins) is returned.  L.at = -1 where the total
-// does not reach it.  Ends in a barrier.
-__device__ u64 scan_find(Lds &L, u64 target) {
+// The first bin at which the running sum reaches target(total) (>= 1), in L.at
+// / before / own, and the target itself; L.at = -1 where the total does not
+// reach it.  Ends in a barrier.
+template <class F>
+__device__ __forceinline__ u64 scan_find(Lds &L, F target_of, u64 &total) {
   const int t = threadIdx.x, wv = t >> 6;
   __syncthreads();
-  const u64 a = L.bin[2 * t], b = L.bin[2 * t + 1], incl = wave_incl(a + b);
+  constexpr int BT = SB / ST;  // bins of a thread
+  u64 e[BT + 1];
+  e[0] = 0;
+#pragma unroll
+  for (int k = 0; k < BT; ++k) e[k + 1] = e[k] + L.bin[BT * t + k];
+  const u64 incl = wave_incl(e[BT]);
   if ((t & 63) == 63) L.wave[wv] = incl;
   if (t == 0) L.at = -1;
   __syncthreads();
-  u64 off = 0, total = 0;
+  static_assert(SW == 16, "the waves' sums in a row of lanes");
+  const u64 v = L.wave[t & 15];
+  total = uni(sum16_64(v));
+  const u64 target = uni(target_of(total)), off = uni(sum16_64((t & 15) < wv ? v : 0ull)) + incl - e[BT];
+  if (off < target && target <= off + e[BT]) {
 #pragma unroll
-  for (int w = 0; w < SW; ++w) {
-    const u64 v = L.wave[w];
-    if (w < wv) off += v;
-    total += v;
-  }
-  const u64 e0 = off + incl - a - b, e1 = e0 + a, e2 = e1 + b;
-  if (e0 < target && target <= e2) {
-    const bool lo = target <= e1;
-    L.at = 2 * t + (lo ? 0 : 1);
-    L.before = lo ? e0 : e1;
-    L.own = lo ? a : b;
+    for (int k = 0; k < BT; ++k)
+      if (off + e[k] < target && target <= off + e[k + 1]) {
+        L.at = BT * t + k;
+        L.before = off + e[k];
+        L.own = e[k + 1] - e[k];
+      }
   }
   __syncthreads();
-  return total;
+  return target;
 }
 
 __device__ __forceinline__ void clear_bins(Lds &L) {
   __syncthreads();
-  L.bin[2 * threadIdx.x] = 0;
-  L.bin[2 * threadIdx.x + 1] = 0;
+#pragma unroll
+  for (int k = 0; k < SB / ST; ++k) L.bin[threadIdx.x + k * ST] = 0;
+  if (threadIdx.x == 0) L.n = 0;
   __syncthreads();
 }
 
-// The tokens of a row, chunk by chunk: lane l of chunk c holds the tokens
-// 256 c + 4 l .. + 3.  A wave takes a run of neighbouring chunks.
-struct Span {
+// Where the passes take the tokens from.  A row in memory, chunk by chunk: lane
+// l of chunk c holds the tokens 256 c + 4 l .. + 3, a wave takes a run of
+// neighbouring chunks, four of them in flight.
+struct Row0 {
   const float *x;
   int vocab, c0, c1;
   __device__ __forceinline__ float4 load(int c) const {
     const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
-    if (i + 4 <= vocab) return ld4u(x + i);
-    float v[4];
+    if (256 * (c + 1) <= vocab) return ld4u(x + i);
+    float e[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = i + e < vocab ? x[i + e] : -INFINITY;
-    return make_float4(v[0], v[1], v[2], v[3]);
+    for (int k = 0; k < 4; ++k) e[k] = i + k < vocab ? x[i + k] : -INFINITY;
+    return make_float4(e[0], e[1], e[2], e[3]);
+  }
+  // f(c, index, values) for each chunk
+  template <class F>
+  __device__ __forceinline__ void chunks(F f) const {
+    for (int c = c0; c < c1; c += 4) {
+      float4 w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) w[j] = load(min(c + j, c1 - 1));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (c + j < c1) f(c + j, 256 * (c + j) + 4 * (int)(threadIdx.x & 63), w[j]);
+    }
   }
   template <class F>
   __device__ __forceinline__ void each(F f) const {
-    for (int c = c0; c < c1; ++c) {
-      const float4 v = load(c);
-      const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
-      f(v.x, i), f(v.y, i + 1), f(v.z, i + 2), f(v.w, i + 3);
-    }
+    chunks([&](int, int i, const float4 &w) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
+  }
+  // L.bin[c]: the sum of f over chunk c
+  template <class F>
+  __device__ __forceinline__ void by_chunk(Lds &L, F f) const {
+    chunks([&](int c, int i, const float4 &w) {
+      const u64 s = (f(w.x, i) + f(w.y, i + 1)) + (f(w.z, i + 2) + f(w.w, i + 3));
+      if (!__any(s != 0)) return;
+      const u64 sum = wave_sum64(s);
+      if ((threadIdx.x & 63) == 0) L.bin[c] = sum;
+    });
+  }
+};
+// The list in LDS, in no order.
+struct List {
+  const Lds *L;
+  int n;
+  template <class F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int m = threadIdx.x; m < n; m += ST) f(L->lz[m], L->li[m]);
+  }
+  template <class F>
+  __device__ __forceinline__ void by_chunk(Lds &L, F f) const {
+    each([&](float z, int i) {
+      const u64 w = f(z, i);
+      if (w) atomicAdd(&L.bin[i >> 8], w);
+    });
   }
 };
 
-// Shortens the cut to the shortest prefix of the order whose sum -- the count
-// of its tokens, or their weight -- reaches target; nothing where the tokens
-// inside the present cut do not reach it.
-template <bool MASS>
-__device__ void cut(Lds &L, const Span &S, Row &R, u64 target) {
-  const float s0 = R.dlim > 0.f ? (float)SB / R.dlim : 0.f;
-  auto bin0 = [&](float z) { return min(SB - 1, (int)(dist(R, z) * s0)); };
-  clear_bins(L);
-  S.each([&](float z, int i) {
-    if (in_cut(R, z, i)) atomicAdd(&L.bin[bin0(z)], MASS ? weight(R, z) : 1ull);
-  });
-  scan_find(L, target);
-  const int b0 = L.at;
-  if (b0 < 0) return;
-  u64 rest = target - L.before;
-  // the range of the bin's keys
-  uint32_t hi = 0u, lo = 0xffffffffu;
-  S.each([&](float z, int i) {
-    if (in_cut(R, z, i) && bin0(z) == b0) {
-      const uint32_t k = key_of(z);
-      hi = max(hi, k);
-      lo = min(lo, k);
-    }
-  });
-#pragma unroll
-  for (int s = 1; s < 64; s <<= 1) {
-    hi = max(hi, (uint32_t)__shfl_xor((int)hi, s));
-    lo = min(lo, (uint32_t)__shfl_xor((int)lo, s));
-  }
-  if ((threadIdx.x & 63) == 0) L.wk[threadIdx.x >> 6] = hi, L.wk[SW + (threadIdx.x >> 6)] = lo;
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < SW; ++w) hi = max(hi, L.wk[w]), lo = min(lo, L.wk[SW + w]);
-  u64 own = L.own;
-  while (hi != lo) {
+// The cut at the first token (in order) of bin b0 at which the running sum
+// reaches target, the bin holding more tokens than can be ranked: by the bits
+// of the logit, then by index.  before: the sum in front of the bin.
+template <bool MASS, class S>
+__device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, Row &R, int b0, u64 rest) {
+  // bounds of the bin's keys
+  const float zl = fmaxf(lo_of(R, b0), R.zcut);
+  uint32_t hi = (uint32_t)uni((int)key_of(hi_of(R, b0))), lo = (uint32_t)uni((int)key_of(zl)), own_shift = 0;
+  u64 own = 0;
+  for (bool more = true; more;) {
     const uint32_t range = hi - lo;
-    const int sh = max(0, 32 - __clz(range) - 11);
+    const int sh = range ? max(0, 32 - __clz((int)range) - 11) : 0;
+    own_shift = (uint32_t)sh;
     clear_bins(L);
-    S.each([&](float z, int i) {
-      const uint32_t k = key_of(z);
-      if (k <= hi && k >= lo && in_cut(R, z, i) && bin0(z) == b0)
-        atomicAdd(&L.bin[(hi - k) >> sh], MASS ? weight(R, z) : 1ull);
+    src.each([&](float z, int i) {
+      if (kept(R, z, i)) {
+        const uint32_t k = key_of(z);
+        if (k <= hi && k >= lo && bin_of(R, z) == b0) atomicAdd(&L.bin[(hi - k) >> sh], MASS ? weight(R, z) : 1ull);
+      }
     });
-    scan_find(L, rest);
-    rest -= L.before;
-    own = L.own;
-    const uint32_t h = hi - ((uint32_t)L.at << sh);
+    u64 total;
+    scan_find(L, [&](u64) { return rest; }, total);
+    rest -= uni(L.before);
+    own = uni(L.own);
+    const uint32_t h = hi - ((uint32_t)uni(L.at) << sh);
     lo = h - lo < (1u << sh) ? lo : h - ((1u << sh) - 1u);
     hi = h;
+    more = own_shift != 0;
   }
-  // the first `need` of the tokens that tie at this key, by index
-  const u64 unit = MASS ? weight(R, hi & 0x80000000u ? __uint_as_float(hi ^ 0x80000000u) : __uint_as_float(~hi)) : 1ull;
-  const u64 need = (rest + unit - 1) / unit;
-  int idx = R.key_cut == hi ? R.idx_cut : 0x7fffffff;
+  // the first `need` of the tokens that tie at this logit, by index
+  const float zc = of_key(hi);
+  const u64 unit = MASS ? weight(R, zc) : 1ull, need = (rest + unit - 1) / unit;
+  int idx = R.zcut == zc ? R.icut : 0x7fffffff;
   if (need * unit < own) {
-    // tokens at the key by chunk, in index order
+    // their number in each chunk
     clear_bins(L);
-    for (int c = S.c0; c < S.c1; ++c) {
-      const float4 v = S.load(c);
-      const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
-      auto hit = [&](float z, int e) { return key_of(z) == hi && in_cut(R, z, i + e); };
-      const int n = __popcll(__ballot(hit(v.x, 0))) + __popcll(__ballot(hit(v.y, 1))) + __popcll(__ballot(hit(v.z, 2))) +
-                    __popcll(__ballot(hit(v.w, 3)));
-      if ((threadIdx.x & 63) == 0) L.bin[c] = (u64)n;
-    }
-    scan_find(L, need);
-    const int c = L.at;
-    if (c >= S.c0 && c < S.c1) {
-      const float4 v = S.load(c);
-      const float z[4] = {v.x, v.y, v.z, v.w};
+    src.by_chunk(L, [&](float z, int i) -> u64 { return z == zc && kept(R, z, i); });
+    u64 total;
+    scan_find(L, [&](u64) { return need; }, total);
+    const int c = uni(L.at);
+    if (c >= row.c0 && c < row.c1) {
+      const float4 w = row.load(c);
+      const float z[4] = {w.x, w.y, w.z, w.w};
       const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
       u64 n = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) n += key_of(z[e]) == hi && in_cut(R, z[e], i + e);
+      for (int e = 0; e < 4; ++e) n += z[e] == zc && kept(R, z[e], i + e);
       u64 k = L.before + wave_incl(n) - n;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        if (key_of(z[e]) == hi && in_cut(R, z[e], i + e) && ++k == need) L.id = i + e;
+        if (z[e] == zc && kept(R, z[e], i + e) && ++k == need) L.id = i + e;
     }
     __syncthreads();
     idx = L.id;
   }
-  R.key_cut = hi;
-  R.idx_cut = idx;
+  R.zcut = uni(zc);
+  R.icut = uni(idx);
+}
+
+// Shortens the cut to the shortest prefix of the order whose sum -- the count
+// of its tokens, or their weight -- reaches target_of(total); nothing where
+// the tokens inside the present cut do not reach it.  Logits below zq need not
+// be counted.
+template <bool MASS, class S, class F>
+__device__ __forceinline__ void cut(Lds &L, const S &src, const Row0 &row, Row &R, float zq, F target_of) {
+  clear_bins(L);
+  src.each([&](float z, int i) {
+    if (!(z < zq) && kept(R, z, i)) atomicAdd(&L.bin[bin_of(R, z)], MASS ? weight(R, z) : 1ull);
+  });
+  u64 total;
+  const u64 target = scan_find(L, target_of, total);
+  const int b0 = uni(L.at);
+  if (b0 < 0) return;
+  const u64 before = uni(L.before);
+  // the bin's tokens (L.n is 0)
+  const float zl = uni(lo_of(R, b0)), zh = uni(hi_of(R, b0));
+  src.each([&](float z, int i) {
+    if (!(z < zl) && !(z > zh) && kept(R, z, i) && bin_of(R, z) == b0) {
+      const int k = atomicAdd(&L.n, 1);
+      if (k < SG) L.gz[k] = z, L.gi[k] = i, L.gw[k] = MASS ? weight(R, z) : 1ull;
+    }
+  });
+  __syncthreads();
+  const int n = uni(L.n);
+  if (n > SG) return cut_wide<MASS>(L, src, row, R, b0, target - before);
+  // eight lanes to a token sum what stands before it
+  static_assert(ST == 8 * SG, "eight lanes to a token");
+  const int m = min((int)threadIdx.x >> 3, n - 1);
+  const float zm = L.gz[m];
+  const int im = L.gi[m];
+  u64 sum = 0;
+  for (int k = threadIdx.x & 7; k < n; k += 8) {
+    const float zk = L.gz[k];
+    if (zk > zm || (zk == zm && L.gi[k] < im)) sum += L.gw[k];
+  }
+  sum = before + sum8_64(sum);
+  if (sum < target && target <= sum + L.gw[m]) L.zcut = zm, L.icut = im;  // the same values from each of its lanes
+  __syncthreads();
+  R.zcut = uni(L.zcut);
+  R.icut = uni(L.icut);
+}
+
+// What a row's settings leave, and the draw, from the tokens of src (those of
+// the row that can be left, at least).
+struct Settings {
+  int k;
+  float p, zq, zp;  // zq: the top k are at least this; zp: min-p leaves nothing below this
+  u64 wmin;         // min-p: the least weight left
+  float u;
+  int32_t *id;
+  float *prob;
+};
+template <class S>
+__device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row &R, const Settings &A) {
+  if (A.k) cut<false>(L, src, row, R, A.zq, [&](u64) { return (u64)A.k; });
+  if (A.p < 1.f)
+    cut<true>(L, src, row, R, -INFINITY, [&](u64 total) {
+      const u64 target = (u64)ceil((double)fmaxf(A.p, 0.f) * (double)total);
+      return target < 1 ? 1ull : target;
+    });
+  auto left = [&](float z, int i) -> u64 {
+    if (z < A.zp || !kept(R, z, i)) return 0;
+    const u64 w = weight(R, z);
+    return w >= A.wmin ? w : 0;
+  };
+  clear_bins(L);
+  src.by_chunk(L, left);
+  // the chunk in which the running sum passes u of the total
+  u64 total;
+  const u64 target = scan_find(L,
+                               [&](u64 total) {
+                                 const u64 x = A.u > 0.f ? (u64)((double)fminf(A.u, 1.f) * (double)total) : 0;
+                                 return (x > total - 1 ? total - 1 : x) + 1;
+                               },
+                               total);
+  const int c = uni(L.at);
+  if (c < row.c0 || c >= row.c1) return;
+  const float4 v = row.load(c);
+  const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
+  const u64 w[4] = {left(v.x, i), left(v.y, i + 1), left(v.z, i + 2), left(v.w, i + 3)};
+  const u64 sum = (w[0] + w[1]) + (w[2] + w[3]);
+  u64 run = L.before + wave_incl(sum) - sum;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if (run < target && target <= run + w[e]) {
+      *A.id = i + e;
+      if (A.prob) *A.prob = (float)((double)w[e] / (double)total);
+    }
+    run += w[e];
+  }
 }
 
 __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   __shared__ Lds L;
-  const int row = blockIdx.x, t = threadIdx.x, wv = t >> 6;
+  const int r = blockIdx.x, t = threadIdx.x, wv = uni(t >> 6);
   const int chunks = (A.vocab + 255) / 256, per = (chunks + SW - 1) / SW;
-  const Span S{A.logits + (size_t)row * A.vocab, A.vocab, min(wv * per, chunks), min((wv + 1) * per, chunks)};
-  // the first token of the order
-  float zv = -INFINITY;
-  int zi = 0x7fffffff;
-  S.each([&](float z, int i) {
-    if (z > zv) zv = z, zi = i;
-  });
-  wave_argmax(zv, zi);
-  if ((t & 63) == 0) L.wv[wv] = zv, L.wi[wv] = zi;
+  const Row0 row{A.logits + (size_t)r * A.vocab, A.vocab, min(wv * per, chunks), min((wv + 1) * per, chunks)};
+  float zt = -INFINITY;  // this thread's maximum
+  row.chunks([&](int, int, const float4 &w) { zt = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), zt); });
+  float zv = wave_max(zt);
+  if ((t & 63) == 0) L.wv[wv] = zv;
+  if (t == 0) L.id = 0x7fffffff, L.ln = 0;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < SW; ++w)
-    if (amax_better(L.wv[w], L.wi[w], zv, zi)) zv = L.wv[w], zi = L.wi[w];
-  const float temp = A.temperature ? A.temperature[row] : 1.f;
-  if (zv == -INFINITY || !(temp > 0.f)) {  // nothing above -inf; greedy
+  zv = uni(row16_max(L.wv[t & 15]));
+  const float temp = A.temperature ? A.temperature[r] : 1.f, mp = A.min_p ? A.min_p[r] : 0.f;
+  if (zv == -INFINITY || !(temp > 0.f) || mp > 1.f) {  // nothing above -inf; greedy; the first token alone is left
+    int at = 0x7fffffff;
+    if (zt == zv && zv != -INFINITY)
+      row.each([&](float z, int i) {
+        if (z == zv) at = min(at, i);
+      });
+    if (at != 0x7fffffff) atomicMin(&L.id, at);
+    __syncthreads();
     if (t == 0) {
-      A.ids[row] = zv == -INFINITY ? 0 : zi;
-      if (A.probs) A.probs[row] = zv == -INFINITY ? 0.f : 1.f;
+      A.ids[r] = zv == -INFINITY ? 0 : L.id;
+      if (A.probs) A.probs[r] = zv == -INFINITY ? 0.f : 1.f;
     }
     return;
   }
   Row R;
   R.zmax = zv;
-  R.first = zi;
-  R.c = 1.4426950408889634074 / (double)temp;
-  R.dlim = fminf((float)((double)WBITS / R.c), 3.402823466e38f);
-  if (R.dlim < 1e-35f) R.dlim = 0.f;  // a temperature below 2e-37: the tokens that tie at the maximum
-  R.key_cut = 0u;
-  R.idx_cut = 0x7fffffff;
-  const int k = A.top_k ? A.top_k[row] : 0;
-  if (k > 0 && k < A.vocab) cut<false>(L, S, R, (u64)k);
-  const float p = A.top_p ? A.top_p[row] : 1.f;
-  if (p < 1.f) {
-    u64 sum = 0;
-    S.each([&](float z, int i) {
-      if (in_cut(R, z, i)) sum += weight(R, z);
-    });
-    sum = wave_incl(sum);
-    __syncthreads();
-    if ((t & 63) == 63) L.wave[wv] = sum;
-    __syncthreads();
-    u64 total = 0;
-#pragma unroll
-    for (int w = 0; w < SW; ++w) total += L.wave[w];
-    const double x = (double)fmaxf(p, 0.f) * (double)total;
-    u64 target = (u64)ceil(x);
-    if (target < 1) target = 1;
-    cut<true>(L, S, R, target);
+  R.dmax = (double)zv;
+  R.c = uni(1.4426950408889634074 / (double)temp);
+  R.slack = uni(fabsf(zv) * 2.4e-7f);
+  float dlim = fminf((float)((double)WBITS / R.c), 3.402823466e38f);
+  if (dlim < 1e-35f) dlim = 0.f;  // a temperature below 2e-37: the tokens that tie at the maximum
+  R.s0 = uni(dlim > 0.f ? (float)SB / dlim : 0.f);
+  R.zcut = uni(fmaxf(zv - dlim, -3.402823466e38f));
+  R.icut = 0x7fffffff;
+  Settings s;
+  s.id = A.ids + r, s.prob = A.probs ? A.probs + r : nullptr;
+  s.u = A.u[r];
+  s.k = A.top_k ? A.top_k[r] : 0;
+  if (s.k < 0 || s.k >= A.vocab) s.k = 0;
+  s.p = A.top_p ? A.top_p[r] : 1.f;
+  s.wmin = mp > 0.f ? (u64)ceil((double)mp * (double)(1ull << WBITS)) : 0;
+  s.zq = s.zp = -INFINITY;
+  if (mp > 0.f && zv != INFINITY) s.zp = uni(zv + logf(mp) * temp * 1.00001f - 1e-5f * temp - R.slack);
+  if (s.k && s.k <= ST) {
+    // k of the threads' maxima lie in the bins up to the k-th one's: so do the
+    // top k
+    clear_bins(L);
+    if (zt >= R.zcut) atomicAdd(&L.bin[bin_of(R, zt)], 1ull);
+    u64 total;
+    scan_find(L, [&](u64) { return (u64)s.k; }, total);
+    if (L.at >= 0) s.zq = uni(lo_of(R, L.at));
   }
-  const float mp = A.min_p ? A.min_p[row] : 0.f;
-  R.wmin = mp > 0.f ? (u64)ceil(fmin((double)mp, 2.0) * (double)(1ull << WBITS)) : 0;
-  auto kept = [&](float z, int i) -> u64 {
-    if (!in_cut(R, z, i)) return 0;
-    const u64 w = weight(R, z);
-    return w >= R.wmin || i == R.first ? w : 0;
-  };
-  clear_bins(L);
-  for (int c = S.c0; c < S.c1; ++c) {
-    const float4 v = S.load(c);
-    const int i = 256 * c + 4 * (int)(t & 63);
-    const u64 w = kept(v.x, i) + kept(v.y, i + 1) + kept(v.z, i + 2) + kept(v.w, i + 3);
-    const u64 s = wave_incl(w);
-    if ((t & 63) == 63) L.bin[c] = s;
-  }
-  // the total, then the chunk in which the running sum passes u of it
-  u64 total = scan_find(L, 1);
-  const float u = A.u[row];
-  u64 target = u > 0.f ? (u64)((double)u * (double)total) : 0;
-  if (target > total - 1) target = total - 1;
-  scan_find(L, target + 1);
-  const int c = L.at;
-  if (c >= S.c0 && c < S.c1) {
-    const float4 v = S.load(c);
-    const int i = 256 * c + 4 * (int)(t & 63);
-    const u64 w[4] = {kept(v.x, i), kept(v.y, i + 1), kept(v.z, i + 2), kept(v.w, i + 3)};
-    const u64 sum = w[0] + w[1] + w[2] + w[3];
-    u64 run = L.before + wave_incl(sum) - sum;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if (run <= target && target < run + w[e]) {
-        A.ids[row] = i + e;
-        if (A.probs) A.probs[row] = (float)((double)w[e] / (double)total);
+  // the tokens that can be left: top-p's total takes all of the top k
+  const float zl = s.p < 1.f ? s.zq : fmaxf(s.zq, s.zp);
+  if (zl > -INFINITY) {
+    row.each([&](float z, int i) {
+      if (!(z < zl) && kept(R, z, i)) {
+        const int m = atomicAdd(&L.ln, 1);
+        if (m < SL) L.lz[m] = z, L.li[m] = i;
       }
-      run += w[e];
-    }
+    });
+    __syncthreads();
+    const int n = uni(L.ln);
+    if (n <= SL) return draw(L, List{&L, n}, row, R, s);
   }
+  draw(L, row, row, R, s);
 }
 
 }  // namespace
