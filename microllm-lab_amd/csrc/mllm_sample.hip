@@ -32,7 +32,7 @@ constexpr int ST = 1024;        // threads
 constexpr int SW = ST / 64;     // waves
 constexpr int SB = 2048;        // bins of a histogram, and chunks of a row at most
 constexpr int SG = 128;         // tokens of a bin that are ranked against each other
-constexpr int SL = 2048;        // tokens that fit the list of those that can be left
+constexpr int SL = 16384;       // tokens that fit the list of those that can be left
 constexpr int kMaxVocab = SB * 256;
 constexpr int WBITS = 44;
 
@@ -67,9 +67,10 @@ __device__ __forceinline__ double uni(double v) { return __longlong_as_double((l
 struct Row {
   float zmax, slack;  // slack: more than two roundings of max - d
   float s0;           // bins per unit of d
-  double dmax, c;     // zmax; log2(e) / T
+  double dmax, c;     // zmax (the largest float for infinity); log2(e) / T
   float zcut;         // kept: z > zcut, or z == zcut and index <= icut (never NaN or -inf)
   int icut;
+  double poly[9];     // weight()'s polynomial, without its constant 1
 };
 
 __device__ __forceinline__ bool kept(const Row &R, float z, int i) {
@@ -85,23 +86,31 @@ __device__ __forceinline__ float hi_of(const Row &R, int b) {
 }
 
 // W of a kept token: 2^t by a polynomial in the distance to the nearest
-// integer (interpolated at Chebyshev nodes, within 8e-16; 1 at 0), the integer
-// in the exponent.
+// integer (interpolated at Chebyshev nodes, within 4e-14; 1 at 0), the integer
+// into the exponent.  Adding 1.5 2^52 + 44 rounds t and leaves its integer + 44
+// in the low word; adding 2^52 leaves the weight's.  (Conversions of doubles to
+// integers, roundings and ldexp take four times an addition.)
+// The coefficients come from scalar registers: from vector registers the
+// compiler copies each before the multiply-add that overwrites the copy.
+__device__ __forceinline__ void set_poly(Row &R) {
+  constexpr double c[9] = {1.0203121063391729e-07, 1.3255224878668817e-06, 1.525268684626772e-05,
+                           1.5403455852453838e-04, 1.3333558179043112e-03, 9.618129159402558e-03,
+                           5.5504108664760424e-02, 2.402265069581299e-01,  6.931471805599453e-01};
+#pragma unroll
+  for (int k = 0; k < 9; ++k) {
+    R.poly[k] = c[k];
+    asm("" : "+s"(R.poly[k]));
+  }
+}
 __device__ __forceinline__ u64 weight(const Row &R, float z) {
-  const double t = z == R.zmax ? 0.0 : ((double)z - R.dmax) * R.c, n = rint(t), f = t - n;
-  double p = 7.070977866508139e-09;
-  p = __builtin_fma(p, f, 1.0205905413765595e-07);
-  p = __builtin_fma(p, f, 1.3215451633221434e-06);
-  p = __builtin_fma(p, f, 1.5252672924850737e-05);
-  p = __builtin_fma(p, f, 1.5403530424776529e-04);
-  p = __builtin_fma(p, f, 1.3333558200794592e-03);
-  p = __builtin_fma(p, f, 9.6181291076186650e-03);
-  p = __builtin_fma(p, f, 5.5504108664651670e-02);
-  p = __builtin_fma(p, f, 2.4022650695910075e-01);
-  p = __builtin_fma(p, f, 6.9314718055994620e-01);
+  constexpr double ROUND = 6755399441055744.0 + WBITS;
+  const double t = ((double)fminf(z, 3.402823466e38f) - R.dmax) * R.c, m = t + ROUND, f = t - (m - ROUND);
+  double p = R.poly[0];
+#pragma unroll
+  for (int k = 1; k < 9; ++k) p = __builtin_fma(p, f, R.poly[k]);
   p = __builtin_fma(p, f, 1.0);
-  const double w = __builtin_ldexp(p, (int)n + WBITS) + 4503599627370496.0;  // 2^52: the integer in the mantissa
-  return (u64)__double_as_longlong(w) & 0xfffffffffffffull;
+  const double w = __hiloint2double(__double2hiint(p) + (__double2loint(m) << 20), __double2loint(p)) + 4503599627370496.0;
+  return (u64)(uint32_t)(__double2hiint(w) & 0xfffff) << 32 | (uint32_t)__double2loint(w);
 }
 
 template <int CTRL>
@@ -201,7 +210,7 @@ __device__ __forceinline__ void clear_bins(Lds &L) {
 
 // Where the passes take the tokens from.  A row in memory, chunk by chunk: lane
 // l of chunk c holds the tokens 256 c + 4 l .. + 3, a wave takes a run of
-// neighbouring chunks, four of them in flight.
+// neighbouring chunks.
 struct Row0 {
   const float *x;
   int vocab, c0, c1;
@@ -213,21 +222,31 @@ struct Row0 {
     for (int k = 0; k < 4; ++k) e[k] = i + k < vocab ? x[i + k] : -INFINITY;
     return make_float4(e[0], e[1], e[2], e[3]);
   }
-  // f(c, index, values) for each chunk
-  template <class F>
+  // f(c, index, values) for each chunk, the next N in flight
+  template <int N = 4, class F>
   __device__ __forceinline__ void chunks(F f) const {
-    for (int c = c0; c < c1; c += 4) {
-      float4 w[4];
+    if (c0 >= c1) return;
+    float4 w[N], next[N];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) w[j] = load(min(c + j, c1 - 1));
+    for (int j = 0; j < N; ++j) next[j] = load(min(c0 + j, c1 - 1));
+    for (int c = c0; c < c1; c += N) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < N; ++j) w[j] = next[j];
+      if (c + N < c1)
+#pragma unroll
+        for (int j = 0; j < N; ++j) next[j] = load(min(c + N + j, c1 - 1));
+#pragma unroll
+      for (int j = 0; j < N; ++j)
         if (c + j < c1) f(c + j, 256 * (c + j) + 4 * (int)(threadIdx.x & 63), w[j]);
     }
   }
-  template <class F>
+  template <int N, class F>
+  __device__ __forceinline__ void fours(F f) const {
+    chunks<N>([&](int, int i, const float4 &w) { f(w, i); });
+  }
+  template <int N = 4, class F>
   __device__ __forceinline__ void each(F f) const {
-    chunks([&](int, int i, const float4 &w) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
+    chunks<N>([&](int, int i, const float4 &w) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
   }
   // L.bin[c]: the sum of f over chunk c
   template <class F>
@@ -240,13 +259,42 @@ struct Row0 {
     });
   }
 };
-// The list in LDS, in no order.
+// The same row in registers, at most NJ chunks to a wave.  The values are made
+// opaque to the compiler in each pass: it would otherwise keep what one pass
+// computes of every token for the next, past the registers there are.
+template <int NJ>
+struct Held {
+  float4 v[NJ];
+  int c0, c1;
+  __device__ __forceinline__ void fetch(const Row0 &row) {
+    c0 = row.c0, c1 = row.c1;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (c0 + j < c1) v[j] = row.load(c0 + j);
+  }
+  template <int N, class F>
+  __device__ __forceinline__ void fours(F f) {
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+      if (c0 + j < c1) {
+        asm volatile("" : "+v"(v[j].x), "+v"(v[j].y), "+v"(v[j].z), "+v"(v[j].w));
+        f(v[j], 256 * (c0 + j) + 4 * lane_id64());
+      }
+  }
+  template <int N, class F>
+  __device__ __forceinline__ void each(F f) {
+    fours<N>([&](const float4 &w, int i) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
+  }
+};
+// The list in LDS, in no order: a thread takes K neighbours (K odd, for the LDS
+// banks), so that the lanes of a wave stand in different chunks of the row.
 struct List {
   const Lds *L;
   int n;
-  template <class F>
+  template <int N = 0, class F>
   __device__ __forceinline__ void each(F f) const {
-    for (int m = threadIdx.x; m < n; m += ST) f(L->lz[m], L->li[m]);
+    const int K = ((n + ST - 1) / ST) | 1, m1 = min(n, ((int)threadIdx.x + 1) * K);
+    for (int m = threadIdx.x * K; m < m1; ++m) f(L->lz[m], L->li[m]);
   }
   template <class F>
   __device__ __forceinline__ void by_chunk(Lds &L, F f) const {
@@ -257,34 +305,52 @@ struct List {
   }
 };
 
+// The bin in which a running sum reaches its target.
+struct Found {
+  int bin;        // -1: it does not reach it
+  u64 rest, own;  // of the target, past what stands before the bin; the bin's sum
+};
+
 // The cut at the first token (in order) of bin b0 at which the running sum
 // reaches target, the bin holding more tokens than can be ranked: by the bits
 // of the logit, then by index.  before: the sum in front of the bin.
 template <bool MASS, class S>
-__device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, Row &R, int b0, u64 rest) {
-  // bounds of the bin's keys
-  const float zl = fmaxf(lo_of(R, b0), R.zcut);
-  uint32_t hi = (uint32_t)uni((int)key_of(hi_of(R, b0))), lo = (uint32_t)uni((int)key_of(zl)), own_shift = 0;
-  u64 own = 0;
-  for (bool more = true; more;) {
-    const uint32_t range = hi - lo;
-    const int sh = range ? max(0, 32 - __clz((int)range) - 11) : 0;
-    own_shift = (uint32_t)sh;
+__device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, Row &R, const Found &F) {
+  const int b0 = F.bin;
+  u64 rest = F.rest, own = F.own;
+  uint32_t hi = 0xffffffffu, lo = 0u;
+  auto member = [&](float z, int i, uint32_t k) { return kept(R, z, i) && k <= hi && k >= lo && bin_of(R, z) == b0; };
+  for (;;) {
+    // the range of the keys that are left; one where they tie
+    uint32_t h = 0u, l = 0xffffffffu;
+    src.each([&](float z, int i) {
+      const uint32_t k = key_of(z);
+      if (member(z, i, k)) h = max(h, k), l = min(l, k);
+    });
+#pragma unroll
+    for (int s = 1; s < 64; s <<= 1) {
+      h = max(h, (uint32_t)__shfl_xor((int)h, s));
+      l = min(l, (uint32_t)__shfl_xor((int)l, s));
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) L.wave[threadIdx.x >> 6] = (u64)h << 32 | l;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < SW; ++w) h = max(h, (uint32_t)(L.wave[w] >> 32)), l = min(l, (uint32_t)L.wave[w]);
+    hi = (uint32_t)uni((int)h), lo = (uint32_t)uni((int)l);
+    if (hi == lo) break;
+    const int sh = max(0, 32 - __clz((int)(hi - lo)) - 11);
     clear_bins(L);
     src.each([&](float z, int i) {
-      if (kept(R, z, i)) {
-        const uint32_t k = key_of(z);
-        if (k <= hi && k >= lo && bin_of(R, z) == b0) atomicAdd(&L.bin[(hi - k) >> sh], MASS ? weight(R, z) : 1ull);
-      }
+      const uint32_t k = key_of(z);
+      if (member(z, i, k)) atomicAdd(&L.bin[(hi - k) >> sh], MASS ? weight(R, z) : 1ull);
     });
     u64 total;
     scan_find(L, [&](u64) { return rest; }, total);
     rest -= uni(L.before);
     own = uni(L.own);
-    const uint32_t h = hi - ((uint32_t)uni(L.at) << sh);
-    lo = h - lo < (1u << sh) ? lo : h - ((1u << sh) - 1u);
-    hi = h;
-    more = own_shift != 0;
+    hi -= (uint32_t)uni(L.at) << sh;
+    lo = hi - lo < (1u << sh) ? lo : hi - ((1u << sh) - 1u);
   }
   // the first `need` of the tokens that tie at this logit, by index
   const float zc = of_key(hi);
@@ -316,21 +382,26 @@ __device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, 
   R.icut = uni(idx);
 }
 
-// Shortens the cut to the shortest prefix of the order whose sum -- the count
-// of its tokens, or their weight -- reaches target_of(total); nothing where
-// the tokens inside the present cut do not reach it.  Logits below zq need not
-// be counted.
+// The bin in which the running sum of the order -- the count of the tokens in
+// the present cut, or their weight -- reaches target_of(total).  Logits below
+// zq need not be counted.
 template <bool MASS, class S, class F>
-__device__ __forceinline__ void cut(Lds &L, const S &src, const Row0 &row, Row &R, float zq, F target_of) {
+__device__ __forceinline__ Found find_bin(Lds &L, S &&src, const Row &R, float zq, F target_of) {
   clear_bins(L);
-  src.each([&](float z, int i) {
+  src.template each<4>([&](float z, int i) {
     if (!(z < zq) && kept(R, z, i)) atomicAdd(&L.bin[bin_of(R, z)], MASS ? weight(R, z) : 1ull);
   });
   u64 total;
   const u64 target = scan_find(L, target_of, total);
-  const int b0 = uni(L.at);
-  if (b0 < 0) return;
-  const u64 before = uni(L.before);
+  return Found{uni(L.at), target - uni(L.before), uni(L.own)};
+}
+
+// Shortens the cut to the token of that bin at which the sum reaches its
+// target.
+template <bool MASS, class S>
+__device__ __forceinline__ void settle(Lds &L, const S &src, const Row0 &row, Row &R, const Found &F) {
+  if (F.bin < 0) return;
+  const int b0 = F.bin;
   // the bin's tokens (L.n is 0)
   const float zl = uni(lo_of(R, b0)), zh = uni(hi_of(R, b0));
   src.each([&](float z, int i) {
@@ -341,7 +412,7 @@ __device__ __forceinline__ void cut(Lds &L, const S &src, const Row0 &row, Row &
   });
   __syncthreads();
   const int n = uni(L.n);
-  if (n > SG) return cut_wide<MASS>(L, src, row, R, b0, target - before);
+  if (n > SG) return cut_wide<MASS>(L, src, row, R, F);
   // eight lanes to a token sum what stands before it
   static_assert(ST == 8 * SG, "eight lanes to a token");
   const int m = min((int)threadIdx.x >> 3, n - 1);
@@ -352,8 +423,8 @@ __device__ __forceinline__ void cut(Lds &L, const S &src, const Row0 &row, Row &
     const float zk = L.gz[k];
     if (zk > zm || (zk == zm && L.gi[k] < im)) sum += L.gw[k];
   }
-  sum = before + sum8_64(sum);
-  if (sum < target && target <= sum + L.gw[m]) L.zcut = zm, L.icut = im;  // the same values from each of its lanes
+  sum = sum8_64(sum);
+  if (sum < F.rest && F.rest <= sum + L.gw[m]) L.zcut = zm, L.icut = im;  // the same values from each of its lanes
   __syncthreads();
   R.zcut = uni(L.zcut);
   R.icut = uni(L.icut);
@@ -369,14 +440,18 @@ struct Settings {
   int32_t *id;
   float *prob;
 };
+__device__ __forceinline__ u64 top_p_target(float p, u64 total) {
+  const u64 target = (u64)ceil((double)fmaxf(p, 0.f) * (double)total);
+  return target < 1 ? 1ull : target;
+}
+// F: top-p's bin, where there is no top-k.
 template <class S>
-__device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row &R, const Settings &A) {
-  if (A.k) cut<false>(L, src, row, R, A.zq, [&](u64) { return (u64)A.k; });
-  if (A.p < 1.f)
-    cut<true>(L, src, row, R, -INFINITY, [&](u64 total) {
-      const u64 target = (u64)ceil((double)fmaxf(A.p, 0.f) * (double)total);
-      return target < 1 ? 1ull : target;
-    });
+__device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row &R, const Settings &A, Found F) {
+  if (A.k) {
+    settle<false>(L, src, row, R, find_bin<false>(L, src, R, A.zq, [&](u64) { return (u64)A.k; }));
+    if (A.p < 1.f) F = find_bin<true>(L, src, R, -INFINITY, [&](u64 total) { return top_p_target(A.p, total); });
+  }
+  if (A.p < 1.f) settle<true>(L, src, row, R, F);
   auto left = [&](float z, int i) -> u64 {
     if (z < A.zp || !kept(R, z, i)) return 0;
     const u64 w = weight(R, z);
@@ -409,13 +484,27 @@ __device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row 
   }
 }
 
+// NJ: chunks of a wave that the passes over the whole row take from registers
+// (0: they read them again).
+template <int NJ>
 __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   __shared__ Lds L;
   const int r = blockIdx.x, t = threadIdx.x, wv = uni(t >> 6);
   const int chunks = (A.vocab + 255) / 256, per = (chunks + SW - 1) / SW;
   const Row0 row{A.logits + (size_t)r * A.vocab, A.vocab, min(wv * per, chunks), min((wv + 1) * per, chunks)};
+  Held<NJ ? NJ : 1> held;
   float zt = -INFINITY;  // this thread's maximum
-  row.chunks([&](int, int, const float4 &w) { zt = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), zt); });
+  if constexpr (NJ > 0) {
+    held.fetch(row);
+    held.template each<0>([&](float z, int) { zt = fmaxf(z, zt); });
+  } else {
+    row.chunks<8>([&](int, int, const float4 &w) { zt = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), zt); });
+  }
+  // all of the row, for the passes that need it
+  auto &whole = [&]() -> auto & {
+    if constexpr (NJ > 0) return held;
+    else return row;
+  }();
   float zv = wave_max(zt);
   if ((t & 63) == 0) L.wv[wv] = zv;
   if (t == 0) L.id = 0x7fffffff, L.ln = 0;
@@ -437,8 +526,9 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
     return;
   }
   Row R;
+  set_poly(R);
   R.zmax = zv;
-  R.dmax = (double)zv;
+  R.dmax = (double)fminf(zv, 3.402823466e38f);
   R.c = uni(1.4426950408889634074 / (double)temp);
   R.slack = uni(fabsf(zv) * 2.4e-7f);
   float dlim = fminf((float)((double)WBITS / R.c), 3.402823466e38f);
@@ -465,19 +555,42 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
     if (L.at >= 0) s.zq = uni(lo_of(R, L.at));
   }
   // the tokens that can be left: top-p's total takes all of the top k
-  const float zl = s.p < 1.f ? s.zq : fmaxf(s.zq, s.zp);
+  Found F{-1, 0, 0};
+  float zl = s.p < 1.f ? s.zq : fmaxf(s.zq, s.zp);
+  int last = SB;
+  if (!s.k && s.p < 1.f) {
+    F = find_bin<true>(L, whole, R, -INFINITY, [&](u64 total) { return top_p_target(s.p, total); });
+    last = F.bin;
+    zl = uni(lo_of(R, last));
+  }
   if (zl > -INFINITY) {
-    row.each([&](float z, int i) {
-      if (!(z < zl) && kept(R, z, i)) {
-        const int m = atomicAdd(&L.ln, 1);
-        if (m < SL) L.lz[m] = z, L.li[m] = i;
+    whole.template fours<6>([&](const float4 &w, int i) {
+      const float z[4] = {w.x, w.y, w.z, w.w};
+      if (!__any(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) >= zl)) return;
+      u64 hit[4];  // the lanes whose token it is
+      int n = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        hit[e] = __ballot(!(z[e] < zl) && kept(R, z[e], i + e) && bin_of(R, z[e]) <= last);
+        n += __popcll(hit[e]);
+      }
+      if (n == 0) return;
+      int m = 0;  // places in the list, taken at once
+      if ((t & 63) == 0) m = atomicAdd(&L.ln, n);
+      m = uni(m);
+      const u64 below = (1ull << (t & 63)) - 1;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int at = m + __popcll(hit[e] & below);
+        if ((hit[e] >> (t & 63) & 1) && at < SL) L.lz[at] = z[e], L.li[at] = i + e;
+        m += __popcll(hit[e]);
       }
     });
     __syncthreads();
     const int n = uni(L.ln);
-    if (n <= SL) return draw(L, List{&L, n}, row, R, s);
+    if (n <= SL) return draw(L, List{&L, n}, row, R, s, F);
   }
-  draw(L, row, row, R, s);
+  draw(L, row, row, R, s, F);
 }
 
 }  // namespace
@@ -489,7 +602,8 @@ extern "C" int mllm_sample(int rows, int vocab, const float *logits, const float
   if (vocab > kMaxVocab) return set_error(MLLM_ERR_UNSUPPORTED, "vocab=%d exceeds %d", vocab, kMaxVocab);
   MLLM_CHECK(logits && u && ids, "null pointer");
   const SampleArgs A{logits, temperature, top_p, min_p, u, top_k, ids, probs, vocab};
-  hipLaunchKernelGGL(k_sample, dim3((unsigned)rows), dim3(ST), 0, reinterpret_cast<hipStream_t>(stream), A);
+  const auto kern = vocab <= 16 * SW * 256 ? k_sample<16> : k_sample<0>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(ST), 0, reinterpret_cast<hipStream_t>(stream), A);
   MLLM_HIP(hipGetLastError());
   return 0;
 }
