@@ -188,9 +188,12 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  *     out[r] (the heads' rows) is NaN.
  *   - Only positions below len[r] count, whatever the slots behind them hold.
  *     Infinities and NaN within it act as in infer.js:461-504.
- * All products and sums are float32.  The workspace is
- * mllm_attn_paged_workspace() bytes, 16-byte aligned, of any contents (NULL
- * where that is 0); calls that may overlap need one each. */
+ * Sums and the products with the values are float32; the queries multiply the
+ * keys as float32 too, with an f16 cache as two f16 pieces (22 bits).  The
+ * workspace is mllm_attn_paged_workspace() bytes, 16-byte aligned (NULL where
+ * that is 0).  Its first 4096 bytes are zero before the first call with it;
+ * every call leaves them so, and calls of other shapes may share it.  Calls
+ * that may overlap need one each. */
 int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, const float *q, const int32_t *seq,
                     const int32_t *len, int max_len, float scale, float *out, void *workspace,
                     uint64_t workspace_bytes, void *stream);

@@ -238,9 +238,12 @@ def run_attn(pool, q, seqs, lens, heads, scale, max_len=None, out=None, ws=None,
     max_len = max(lens) if max_len is None else max_len
     out = torch.full((R, heads * pool.hd), 7.0, device="cuda") if out is None else out
     n = abi.lib().mllm_attn_paged_workspace(kv, R, heads, max_len)
-    ws = torch.full((max(n, 16),), 255, dtype=torch.uint8, device="cuda")  # NaN, where it were read
+    if ws is None:
+        ws = torch.full((max(n, 4096),), 255, dtype=torch.uint8, device="cuda")  # NaN, where a part were read unwritten
+        ws[:4096] = 0
     abi.call("mllm_attn_paged", kv, R, heads, p(dq), p(ds), p(dl), max_len, scale, p(out), p(ws), n, stream)
     torch.cuda.synchronize()
+    assert not bool(ws[:4096].any())
     return out.cpu().numpy().reshape(R, heads, pool.hd)
 
 
@@ -412,6 +415,33 @@ def test_attn_shared_pages_and_speculation_rows():
 
 
 @gpu
+def test_attn_calls_of_other_shapes_share_a_workspace():
+    g = torch.Generator().manual_seed(20)
+    rng = np.random.default_rng(20)
+    ws = torch.zeros(64 << 20, dtype=torch.uint8, device="cuda")
+    for heads, kvh, hd, lens in ((8, 2, 64, [900, 300]), (40, 5, 32, [400] * 30), (4, 4, 128, [5000]), (8, 2, 64, [100, 900])):
+        pool = Pool(g, kvh, hd, 16, len(lens), -(-max(lens) // 16), "f16")
+        q = rng.standard_normal((len(lens), heads, hd)).astype(np.float32)
+        o = run_attn(pool, q, None, lens, heads, 0.125, ws=ws)
+        ref, tol = ref_attn(q, pool, range(len(lens)), lens, heads, 0.125)
+        assert (np.abs(o - ref) <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-30, 1e-6, 1.0, 3e4, 1e9])
+@pytest.mark.parametrize("storage", ["f16", "bf16"])
+def test_attn_queries_of_any_size(storage, size):
+    """Queries far from 1, with elements of very different size in a head."""
+    g = torch.Generator().manual_seed(21)
+    rng = np.random.default_rng(21)
+    pool = Pool(g, 2, 64, 16, 1, 20, storage)
+    q = (size * rng.standard_normal((1, 6, 64)) * 2.0 ** rng.uniform(-12, 0, (1, 6, 64))).astype(np.float32)
+    o = run_attn(pool, q, None, [310], 6, 1.0 / size)
+    ref, tol = ref_attn(q, pool, [0], [310], 6, float(np.float32(1.0 / size)))
+    assert (np.abs(o - ref) <= tol).all()
+
+
+@gpu
 def test_offsets_past_32_bits():
     """Pages 5 GiB apart: rotation writes them and attention reads them."""
     heads, kvh, hd, page = 4, 2, 64, 16
@@ -430,7 +460,7 @@ def test_offsets_past_32_bits():
     out = torch.empty(1, heads * hd, device="cuda")
     ln = torch.tensor([n], dtype=torch.int32, device="cuda")
     nb = abi.lib().mllm_attn_paged_workspace(kv, 1, heads, n)
-    ws = torch.empty(max(nb, 16), dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(max(nb, 16), dtype=torch.uint8, device="cuda")
     abi.call("mllm_attn_paged", kv, 1, heads, p(q[3:4]), None, p(ln), n, 0.125, p(out), p(ws), nb, None)
     torch.cuda.synchronize()
     assert torch.equal(q, dx[:, :heads * hd])
@@ -540,7 +570,7 @@ class PagedLlama:
             abi.call("mllm_rope_kv_paged", kv, T, c.n_heads, p(qkv), p(ds), p(dp), p(self.freq), self.hd, 0, None, None, 0.0,
                      p(q), None)
             n = abi.lib().mllm_attn_paged_workspace(kv, T, c.n_heads, max(pos) + 1)
-            ws = torch.empty(max(n, 16), dtype=torch.uint8, device="cuda")
+            ws = torch.zeros(max(n, 16), dtype=torch.uint8, device="cuda")
             abi.call("mllm_attn_paged", kv, T, c.n_heads, p(q), p(ds), p(ln), max(pos) + 1, 1.0 / math.sqrt(self.hd), p(o),
                      p(ws), n, None)
             x = x + self.gemm(b + "attn.proj", o)
