@@ -180,7 +180,7 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  * (n_heads a multiple of n_kv_heads), and row r attends to positions 0 ..
  * len[r] - 1 of sequence seq[r] (seq NULL: sequence r).  Several rows may have
  * one sequence: a speculation pass is a row per token, each one longer.
- * max_len bounds every len (at most page_size * table_cols); the work is split
+ * q is 16-byte aligned.  max_len bounds every len (at most page_size * table_cols); the work is split
  * over it, so a host passes the longest it knows of.
  *   - len[r] = 0: out[r] is 0.  A sequence outside [0, sequences) is padding:
  *     out[r] is left as it was.
@@ -191,7 +191,7 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  * Sums and the products with the values are float32; the queries multiply the
  * keys as float32 too, with an f16 cache as two f16 pieces (22 bits).  The
  * workspace is mllm_attn_paged_workspace() bytes, 16-byte aligned (NULL where
- * that is 0).  Its first 4096 bytes are zero before the first call with it;
+ * that is 0).  Its first 16384 bytes are zero before the first call with it;
  * every call leaves them so, and calls of other shapes may share it.  Calls
  * that may overlap need one each. */
 int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, const float *q, const int32_t *seq,

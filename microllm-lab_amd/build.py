@@ -38,11 +38,13 @@ CONVERT_BIN = os.path.join(PKG, "convert", "pgw_convert")
 NAPI_OUT = os.path.join(PKG, "js", "mllm_napi.node")
 
 HIP_SOURCES = ["mllm_ops.hip", "mllm_engine.hip", "mllm_prefill.hip", "mllm_generic.hip",
-               "mllm_gprompt.hip", "mllm_paged.hip", "mllm_sample.hip"]
+               "mllm_gprompt.hip", "mllm_paged.hip", "mllm_attn_f32.hip", "mllm_attn_f16.hip",
+               "mllm_attn_bf16.hip", "mllm_sample.hip"]
 # per-source flags: the prefill kernels consume their matrix-core results in
 # VALU epilogues, so the results go to VGPRs (no AGPR-to-VGPR copies)
-EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("mllm_ops.hip", "mllm_prefill.hip", "mllm_gprompt.hip",
-                                                                              "mllm_paged.hip")}
+EXTRA_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"]
+               for f in ("mllm_ops.hip", "mllm_prefill.hip", "mllm_gprompt.hip", "mllm_attn_f32.hip",
+                         "mllm_attn_f16.hip", "mllm_attn_bf16.hip")}
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("MLLM_OFFLOAD_ARCH", "gfx950")
 HIP_FLAGS = [

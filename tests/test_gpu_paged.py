@@ -239,11 +239,11 @@ def run_attn(pool, q, seqs, lens, heads, scale, max_len=None, out=None, ws=None,
     out = torch.full((R, heads * pool.hd), 7.0, device="cuda") if out is None else out
     n = abi.lib().mllm_attn_paged_workspace(kv, R, heads, max_len)
     if ws is None:
-        ws = torch.full((max(n, 4096),), 255, dtype=torch.uint8, device="cuda")  # NaN, where a part were read unwritten
-        ws[:4096] = 0
+        ws = torch.full((max(n, 16384),), 255, dtype=torch.uint8, device="cuda")  # NaN, where a part were read unwritten
+        ws[:16384] = 0
     abi.call("mllm_attn_paged", kv, R, heads, p(dq), p(ds), p(dl), max_len, scale, p(out), p(ws), n, stream)
     torch.cuda.synchronize()
-    assert not bool(ws[:4096].any())
+    assert not bool(ws[:16384].any())
     return out.cpu().numpy().reshape(R, heads, pool.hd)
 
 
@@ -280,7 +280,7 @@ def test_attn_many_rows_take_one_part():
     g = torch.Generator().manual_seed(11)
     rng = np.random.default_rng(11)
     pool = Pool(g, 4, 64, 16, 300, 9, "f16")
-    lens = [int(v) for v in rng.integers(0, 140, 300)]
+    lens = [int(v) for v in rng.integers(0, 140, 300)]  # a part is 256 positions at least
     q = rng.standard_normal((300, 8, 64)).astype(np.float32)
     assert abi.lib().mllm_attn_paged_workspace(pool.desc(), 300, 8, max(lens)) == 0
     o = run_attn(pool, q, None, lens, 8, 0.125)

@@ -62,7 +62,7 @@ def test_rope_null_pages():
 
 
 @pytest.mark.parametrize("over", [
-    dict(rows=0), dict(rows=-4), dict(heads=0), dict(heads=5), dict(q=None), dict(ln=None), dict(out=None),
+    dict(rows=0), dict(rows=-4), dict(heads=0), dict(heads=5), dict(q=None), dict(q=B + 4), dict(ln=None), dict(out=None),
     dict(max_len=-1), dict(max_len=65), dict(seq=None, rows=5), dict(rows=1 << 30, heads=1 << 10)])
 def test_attn_refusals(over):
     assert attn(pages(), **over) == INVALID
