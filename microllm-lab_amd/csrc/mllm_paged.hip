@@ -17,107 +17,133 @@ struct RopeArgs {
   const float *qkv, *inv_freq, *q_gain, *k_gain;
   const int32_t *seq, *pos;
   float *q;
-  int n_heads, rot, lph, lg_lph, per_wg, n_wg;  // lanes per head (a power of two), heads per workgroup, workgroups per token
+  int n_heads, rot, lg_lph;  // 2^lg_lph lanes per head
   int interleaved;
   float eps;
 };
 
-// A token's heads, lph lanes to each: lane s holds the four pairs 4s .. 4s + 3.
+// A token's heads, lph lanes to each: lane s takes the same four pairs of every
+// head that its group of lanes reaches, so that their angles are formed once.
 // Pair p is rotated below rot / 2 -- elements (p, p + rot/2), or (2p, 2p + 1)
-// interleaved -- and passes through above, as elements (2p, 2p + 1).  VEC: rot
-// is a multiple of 8, so a lane's pairs are two runs of four floats.
+// interleaved.  VEC (rot a multiple of 8): a lane's elements are two runs of
+// four, each side by side with the next lane's -- p = 4s .. 4s + 3 in halves,
+// and 4s .., hd/2 + 4s .. of what is interleaved or not rotated.  Otherwise a
+// lane's pairs are 4s .. 4s + 3, element by element.
+//
+// What bounds it: the bytes, at the rate of a copy.  8000 tokens with 48 heads
+// of 128 (360 MB), us: runs of eight elements a lane, which touch every cache
+// line twice, 124; runs of four 75, three heads of a lane in flight 88, three
+// times the threads 98; loads and stores past the caches, whose readers sit
+// behind another L2, 70 (5.2 TB/s; a large copy moves 4.8).
 //
 // The angle is formed in double and in turns: a position of 2^20 keeps 2^-33
 // of a turn, where a float product would keep 2^-4.
 template <class KV, bool VEC>
 __global__ __launch_bounds__(WG) void k_rope_kv(RopeArgs A) {
-  const int token = blockIdx.x / A.n_wg, part = blockIdx.x - token * A.n_wg;
-  const int s = threadIdx.x & (A.lph - 1), head = part * A.per_wg + (threadIdx.x >> A.lg_lph);
-  const int nh = A.n_heads, nkv = A.P.n_kv, hd = A.P.hd, rows = nh + 2 * nkv;
-  if ((int)(threadIdx.x >> A.lg_lph) >= A.per_wg || head >= rows) return;  // whole heads
+  const int token = blockIdx.x, lph = 1 << A.lg_lph, s = threadIdx.x & (lph - 1);
+  const int nh = A.n_heads, nkv = A.P.n_kv, hd = A.P.hd, rows = nh + 2 * nkv, step = (int)blockDim.x >> A.lg_lph;
+  const float *row = A.qkv + (size_t)token * rows * hd;
+  const bool in = 8 * s < hd;
+  const int half = A.rot >> 1;
+  // the lane's pair j, where it is rotated (2 pair < rot)
+  auto pair = [&](int j) { return VEC && A.interleaved ? (j < 2 ? 2 * s + j : (hd >> 2) + 2 * s + j - 2) : 4 * s + j; };
+  // r: a head of the queries or keys.  Element e of pair j, without runs
+  auto at1 = [&](bool r, int j, int e) {
+    const int p = 4 * s + j;
+    return r && 2 * p < A.rot && !A.interleaved ? p + e * half : 2 * p + e;
+  };
+  // the runs: halves of the rotated part, or of what passes through behind it
+  auto halves = [&](bool r) { return r && !A.interleaved && 8 * s < A.rot; };
+  auto run0 = [&](bool r) { return r && !A.interleaved && 8 * s >= A.rot ? 4 * s + half : 4 * s; };
+  auto run1 = [&](bool r) {
+    return !r || A.interleaved ? (hd >> 1) + 4 * s : 8 * s < A.rot ? half + 4 * s : (hd >> 1) + 4 * s;
+  };
+  auto at = [&](bool r, int j, int e) {
+    if (!VEC) return at1(r, j, e);
+    if (halves(r)) return e ? run1(r) + j : run0(r) + j;
+    return (j < 2 ? run0(r) : run1(r)) + 2 * (j & 1) + e;
+  };
+  float a[4], b[4];  // the pairs' elements
+  auto load = [&](int head, float (&u)[4], float (&w)[4]) {
+    const bool r = head < nh + nkv;
+    const float *x = row + (size_t)head * hd;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) u[j] = w[j] = 0.f;
+    if (!in || head >= rows) return;
+    if (VEC) {
+      const v4f f = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(x + run0(r)));
+      const v4f g = __builtin_nontemporal_load(reinterpret_cast<const v4f *>(x + run1(r)));
+      const bool h = halves(r);
+      u[0] = f.x, u[1] = h ? f.y : f.z, u[2] = h ? f.z : g.x, u[3] = h ? f.w : g.z;
+      w[0] = h ? g.x : f.y, w[1] = h ? g.y : f.w, w[2] = h ? g.z : g.y, w[3] = g.w;
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = x[at1(r, j, 0)], w[j] = x[at1(r, j, 1)];
+    }
+  };
+  const int first = threadIdx.x >> A.lg_lph;
+  load(first, a, b);
   const int seq = A.seq ? A.seq[token] : token, pos = A.pos[token];
   if (seq < 0 || seq >= A.P.sequences || pos < 0) return;  // padding
-  const bool in = 8 * s < hd, turned = head < nh + nkv && 8 * s < A.rot;
-  const float *x = A.qkv + ((size_t)token * rows + head) * hd;
-  // element e of the lane's pair j
-  auto at = [&](int j, int e) {
-    const int p = 4 * s + j;
-    const bool r = head < nh + nkv && 2 * p < A.rot;
-    return r && !A.interleaved ? p + e * (A.rot >> 1) : 2 * p + e;
-  };
-  const bool halves = turned && !A.interleaved;
-  const int o0 = halves ? 4 * s : 8 * s, o1 = halves ? 4 * s + (A.rot >> 1) : 8 * s + 4;
-  float a[4], b[4];  // the pairs' elements
-  if (!in) {
+  // the slot, if there is one
+  const int col = page_of(A.P, pos), slot = pos - col * A.P.page_size;
+  int page = -1;
+  if (col < A.P.table_cols) page = A.P.table[(size_t)seq * A.P.table_cols + col];
+  const bool placed = page >= 0 && page < A.P.pages;
+  const int64_t place = placed ? page * A.P.page_stride + slot * A.P.row_stride : 0;
+  float sn[4], cs[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = b[j] = 0.f;
-  } else if (VEC) {
-    const float4 u = *reinterpret_cast<const float4 *>(x + o0), w = *reinterpret_cast<const float4 *>(x + o1);
-    if (halves) {
-      a[0] = u.x, a[1] = u.y, a[2] = u.z, a[3] = u.w, b[0] = w.x, b[1] = w.y, b[2] = w.z, b[3] = w.w;
-    } else {
-      a[0] = u.x, b[0] = u.y, a[1] = u.z, b[1] = u.w, a[2] = w.x, b[2] = w.y, a[3] = w.z, b[3] = w.w;
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) a[j] = x[at(j, 0)], b[j] = x[at(j, 1)];
-  }
-  const float *gain = head < nh ? A.q_gain : head < nh + nkv ? A.k_gain : nullptr;
-  if (gain) {
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(a[j], a[j], __builtin_fmaf(b[j], b[j], ss));
-    for (int m = 1; m < A.lph; m <<= 1) ss += __shfl_xor(ss, m);
-    const float inv = 1.0f / sqrtf(ss / (float)hd + A.eps);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (in) a[j] = a[j] * inv * gain[at(j, 0)], b[j] = b[j] * inv * gain[at(j, 1)];
-  }
-  if (!in) return;
-  if (turned) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int p = 4 * s + j;
-      if (2 * p < A.rot) {
-        const double t = (double)pos * ((double)A.inv_freq[p] * 0.15915494309189533577);  // turns
-        float sn, cs;
-        sincospif((float)(2.0 * (t - rint(t))), &sn, &cs);
-        const float u = a[j], w = b[j];
-        a[j] = u * cs - w * sn;
-        b[j] = w * cs + u * sn;
-      }
+  for (int j = 0; j < 4; ++j) {
+    sn[j] = 0.f, cs[j] = 1.f;
+    if (in && 2 * pair(j) < A.rot) {
+      const double t = (double)pos * ((double)A.inv_freq[pair(j)] * 0.15915494309189533577);  // turns
+      sincospif((float)(2.0 * (t - rint(t))), &sn[j], &cs[j]);
     }
   }
-  auto store = [&](auto *to, auto put) {
+  auto store = [&](bool r, const float (&u)[4], const float (&w)[4], auto *to, auto put) {
     using T = decltype(put(0.f));
     if (VEC) {
       typedef T v4 __attribute__((ext_vector_type(4)));
-      v4 u, w;
-      if (halves) {
-        u = v4{put(a[0]), put(a[1]), put(a[2]), put(a[3])};
-        w = v4{put(b[0]), put(b[1]), put(b[2]), put(b[3])};
-      } else {
-        u = v4{put(a[0]), put(b[0]), put(a[1]), put(b[1])};
-        w = v4{put(a[2]), put(b[2]), put(a[3]), put(b[3])};
-      }
-      *reinterpret_cast<v4 *>(to + o0) = u;
-      *reinterpret_cast<v4 *>(to + o1) = w;
+      const bool h = halves(r);
+      const float f[8] = {u[0], h ? u[1] : w[0], h ? u[2] : u[1], h ? u[3] : w[1],
+                          h ? w[0] : u[2], h ? w[1] : w[2], h ? w[2] : u[3], w[3]};
+      __builtin_nontemporal_store(v4{put(f[0]), put(f[1]), put(f[2]), put(f[3])}, reinterpret_cast<v4 *>(to + run0(r)));
+      __builtin_nontemporal_store(v4{put(f[4]), put(f[5]), put(f[6]), put(f[7])}, reinterpret_cast<v4 *>(to + run1(r)));
     } else {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) to[at(j, 0)] = put(a[j]), to[at(j, 1)] = put(b[j]);
+      for (int j = 0; j < 4; ++j) to[at1(r, j, 0)] = put(u[j]), to[at1(r, j, 1)] = put(w[j]);
     }
   };
-  if (head < nh) {
-    store(A.q + ((size_t)token * nh + head) * hd, KvF32::put);
-    return;
+  for (int head = first; head < rows; head += step) {
+    if (head != first) load(head, a, b);
+    const bool r = head < nh + nkv;
+    const float *gain = head < nh ? A.q_gain : r ? A.k_gain : nullptr;
+    if (gain) {
+      float ss = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) ss = __builtin_fmaf(a[j], a[j], __builtin_fmaf(b[j], b[j], ss));
+      for (int m = 1; m < lph; m <<= 1) ss += __shfl_xor(ss, m);
+      const float inv = 1.0f / sqrtf(ss / (float)hd + A.eps);
+      if (in)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = a[j] * inv * gain[at(r, j, 0)], b[j] = b[j] * inv * gain[at(r, j, 1)];
+    }
+    if (!in) continue;
+    if (r)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (2 * pair(j) < A.rot) {
+          const float u = a[j], w = b[j];
+          a[j] = u * cs[j] - w * sn[j];
+          b[j] = w * cs[j] + u * sn[j];
+        }
+    if (head < nh) {
+      store(r, a, b, A.q + ((size_t)token * nh + head) * hd, KvF32::put);
+    } else if (placed) {
+      typename KV::T *pool = static_cast<typename KV::T *>(r ? A.P.k : A.P.v);
+      store(r, a, b, pool + place + (r ? head - nh : head - nh - nkv) * A.P.head_stride, KV::put);
+    }
   }
-  const int col = page_of(A.P, pos), slot = pos - col * A.P.page_size;
-  if (col >= A.P.table_cols) return;
-  const int page = A.P.table[(size_t)seq * A.P.table_cols + col];
-  if (page < 0 || page >= A.P.pages) return;
-  const int kvh = head < nh + nkv ? head - nh : head - nh - nkv;
-  typename KV::T *pool = static_cast<typename KV::T *>(head < nh + nkv ? A.P.k : A.P.v);
-  store(pool + page * A.P.page_stride + kvh * A.P.head_stride + slot * A.P.row_stride, KV::put);
 }
 
 // ---------------------------------------------------------------- host side
@@ -207,7 +233,7 @@ int attn_shape(const mllm_kv_pages *kv, const Pages &P, int rows, int n_heads, i
   pl->tiles = (pl->rep + aq - 1) / aq;
   pl->units = (int64_t)rows * P.n_kv * pl->tiles;
   pl->pos_bytes = 2 * P.hd * (kv->storage == MLLM_F32 ? 4 : 2);
-  MLLM_CHECK(pl->units < (1ll << 31) && (int64_t)rows * n_heads < (1ll << 31), "%d rows of %d heads exceed a launch", rows,
+  MLLM_CHECK(pl->units * 64 * AW < (1ll << 32), "%d rows of %d heads exceed a launch", rows,
              n_heads);
   attn_plan(pl->units, max_len, pl->pos_bytes, &pl->chunk, &pl->splits);
   pl->bytes = pl->splits > 1 ? kCounters * sizeof(unsigned) +
@@ -233,15 +259,14 @@ extern "C" int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_hea
   A.qkv = qkv, A.inv_freq = inv_freq, A.q_gain = q_gain, A.k_gain = k_gain;
   A.seq = seq, A.pos = pos, A.q = q;
   A.n_heads = n_heads, A.rot = rot, A.interleaved = interleaved != 0, A.eps = eps;
-  A.lph = 4, A.lg_lph = 2;
-  while (8 * A.lph < A.P.hd) A.lph <<= 1, ++A.lg_lph;
+  A.lg_lph = 2;
+  while (8 << A.lg_lph < A.P.hd) ++A.lg_lph;
   const int64_t heads = (int64_t)n_heads + 2 * (int64_t)A.P.n_kv;
-  const int fit = WG >> A.lg_lph;
-  A.n_wg = (int)((heads + fit - 1) / fit);
-  A.per_wg = (int)((heads + A.n_wg - 1) / A.n_wg);
-  MLLM_CHECK(heads < (1 << 20) && (int64_t)tokens * A.n_wg < (1ll << 31), "%d tokens of %lld heads exceed a launch",
-             tokens, (long long)heads);
-  const dim3 grid((unsigned)(tokens * A.n_wg)), block((unsigned)((A.per_wg * A.lph + 63) & ~63));
+  MLLM_CHECK(heads < (1 << 20), "%lld heads", (long long)heads);
+  const int threads = heads << A.lg_lph < WG ? (int)(heads << A.lg_lph) : WG;  // whole waves
+  const dim3 grid((unsigned)tokens), block((unsigned)((threads + 63) & ~63));
+  MLLM_CHECK((uint64_t)tokens * block.x < (1ull << 32), "%d tokens of %lld heads exceed a launch", tokens,
+             (long long)heads);
   const bool vec = rot % 8 == 0;
   const auto kern = kv->storage == MLLM_F32   ? (vec ? k_rope_kv<KvF32, true> : k_rope_kv<KvF32, false>)
                     : kv->storage == MLLM_F16 ? (vec ? k_rope_kv<KvF16, true> : k_rope_kv<KvF16, false>)

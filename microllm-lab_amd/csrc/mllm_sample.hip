@@ -600,6 +600,7 @@ extern "C" int mllm_sample(int rows, int vocab, const float *logits, const float
                            void *stream) {
   MLLM_CHECK(rows > 0 && vocab > 0, "invalid shape rows=%d vocab=%d", rows, vocab);
   if (vocab > kMaxVocab) return set_error(MLLM_ERR_UNSUPPORTED, "vocab=%d exceeds %d", vocab, kMaxVocab);
+  MLLM_CHECK((int64_t)rows * ST < (1ll << 32), "%d rows exceed a launch", rows);
   MLLM_CHECK(logits && u && ids, "null pointer");
   const SampleArgs A{logits, temperature, top_p, min_p, u, top_k, ids, probs, vocab};
   const auto kern = vocab <= 16 * SW * 256 ? k_sample<16> : k_sample<0>;

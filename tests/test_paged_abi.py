@@ -63,7 +63,7 @@ def test_rope_null_pages():
 
 @pytest.mark.parametrize("over", [
     dict(rows=0), dict(rows=-4), dict(heads=0), dict(heads=5), dict(q=None), dict(q=B + 4), dict(ln=None), dict(out=None),
-    dict(max_len=-1), dict(max_len=65), dict(seq=None, rows=5), dict(rows=1 << 30, heads=1 << 10)])
+    dict(max_len=-1), dict(max_len=65), dict(seq=None, rows=5), dict(rows=1 << 30, heads=1 << 10), dict(rows=1 << 23)])
 def test_attn_refusals(over):
     assert attn(pages(), **over) == INVALID
 
@@ -79,7 +79,7 @@ def test_attn_workspace_is_checked():
 
 
 @pytest.mark.parametrize("over,code", [
-    (dict(rows=0), INVALID), (dict(vocab=0), INVALID), (dict(vocab=524289), UNSUPPORTED), (dict(logits=None), INVALID),
+    (dict(rows=0), INVALID), (dict(vocab=0), INVALID), (dict(rows=1 << 22), INVALID), (dict(vocab=524289), UNSUPPORTED), (dict(logits=None), INVALID),
     (dict(u=None), INVALID), (dict(ids=None), INVALID)])
 def test_sample_refusals(over, code):
     a = dict(rows=2, vocab=100, logits=B, u=B, ids=B)
