@@ -19,15 +19,21 @@ namespace {
 //
 // The order of the tokens is: larger logit first, equal ones by index.  top-k
 // and top-p both keep a prefix of it -- the shortest whose count reaches k, or
-// whose weight reaches top_p of the total -- and so does min-p.  No sort: the
-// tokens' counts or weights are summed into 2048 bins of equal width in d (LDS
-// atomics on 64-bit integers), the bin in which the running sum passes its
-// target is gathered, and each of its tokens counts what stands before it.  A
-// bin of more than 128 tokens (ties, a wide spread of logits) is split further
-// by the bits of the logit, at most three times, and then by index.
-//
-// The draw itself sums the kept weights by 256-token chunks in index order and
-// takes the first token whose running sum is more than u of the total.
+// whose weight reaches top_p of the total -- and so does min-p.  No sort:
+//   1 the maximum, of the row, of each thread and of each 1024 tokens;
+//   2 a bound on the logits that can be left: the k-th of the threads' maxima
+//     for top-k, the least weight for min-p; for top-p alone the weights of all
+//     tokens are summed into 2048 bins of equal width in d (LDS atomics on
+//     64-bit integers), and the bin in which the sum passes its target bounds
+//     them;
+//   3 the tokens within the bound are listed in LDS, from the 1024s whose
+//     maximum is;
+//   4 128 tokens or fewer are ranked each against each, and drawn from; a longer
+//     list goes through histograms as in 2, whose last bin is ranked so (a bin of
+//     more than 128 tokens is split by the bits of its logits, at most three
+//     times, and then by index);
+//   5 the kept weights are summed by chunks in index order, and the first token
+//     whose running sum is more than u of the total is drawn.
 constexpr int ST = 1024;        // threads
 constexpr int SW = ST / 64;     // waves
 constexpr int SB = 2048;        // bins of a histogram, and chunks of a row at most
@@ -148,13 +154,13 @@ __device__ __forceinline__ u64 wave_incl(u64 v) {  // inclusive scan over the la
 
 struct Lds {
   u64 bin[SB];
+  float top[SB / 4];  // the maxima of the waves' groups of four chunks
   u64 wave[SW];
   // the bin that scan_find has found: its number, the sum before it, its own sum
   int at;
   u64 before, own;
-  // the tokens that can be left
-  float lz[SL];
-  int li[SL];
+  // the tokens that can be left: logits' bits and indices
+  uint2 list[SL];
   int ln;
   // the tokens of a bin
   u64 gw[SG];
@@ -211,9 +217,10 @@ __device__ __forceinline__ void clear_bins(Lds &L) {
 // Where the passes take the tokens from.  A row in memory, chunk by chunk: lane
 // l of chunk c holds the tokens 256 c + 4 l .. + 3, a wave takes a run of
 // neighbouring chunks.
-struct Row0 {
+struct Tokens {
   const float *x;
   int vocab, c0, c1;
+  int g0;  // its first group in Lds::top
   __device__ __forceinline__ float4 load(int c) const {
     const int i = 256 * c + 4 * (int)(threadIdx.x & 63);
     if (256 * (c + 1) <= vocab) return ld4u(x + i);
@@ -240,13 +247,9 @@ struct Row0 {
         if (c + j < c1) f(c + j, 256 * (c + j) + 4 * (int)(threadIdx.x & 63), w[j]);
     }
   }
-  template <int N, class F>
-  __device__ __forceinline__ void fours(F f) const {
-    chunks<N>([&](int, int i, const float4 &w) { f(w, i); });
-  }
-  template <int N = 4, class F>
+  template <class F>
   __device__ __forceinline__ void each(F f) const {
-    chunks<N>([&](int, int i, const float4 &w) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
+    chunks([&](int, int i, const float4 &w) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
   }
   // L.bin[c]: the sum of f over chunk c
   template <class F>
@@ -259,42 +262,18 @@ struct Row0 {
     });
   }
 };
-// The same row in registers, at most NJ chunks to a wave.  The values are made
-// opaque to the compiler in each pass: it would otherwise keep what one pass
-// computes of every token for the next, past the registers there are.
-template <int NJ>
-struct Held {
-  float4 v[NJ];
-  int c0, c1;
-  __device__ __forceinline__ void fetch(const Row0 &row) {
-    c0 = row.c0, c1 = row.c1;
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (c0 + j < c1) v[j] = row.load(c0 + j);
-  }
-  template <int N, class F>
-  __device__ __forceinline__ void fours(F f) {
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      if (c0 + j < c1) {
-        asm volatile("" : "+v"(v[j].x), "+v"(v[j].y), "+v"(v[j].z), "+v"(v[j].w));
-        f(v[j], 256 * (c0 + j) + 4 * lane_id64());
-      }
-  }
-  template <int N, class F>
-  __device__ __forceinline__ void each(F f) {
-    fours<N>([&](const float4 &w, int i) { f(w.x, i), f(w.y, i + 1), f(w.z, i + 2), f(w.w, i + 3); });
-  }
-};
 // The list in LDS, in no order: a thread takes K neighbours (K odd, for the LDS
 // banks), so that the lanes of a wave stand in different chunks of the row.
 struct List {
   const Lds *L;
   int n;
-  template <int N = 0, class F>
+  template <class F>
   __device__ __forceinline__ void each(F f) const {
     const int K = ((n + ST - 1) / ST) | 1, m1 = min(n, ((int)threadIdx.x + 1) * K);
-    for (int m = threadIdx.x * K; m < m1; ++m) f(L->lz[m], L->li[m]);
+    for (int m = threadIdx.x * K; m < m1; ++m) {
+      const uint2 e = L->list[m];
+      f(__uint_as_float(e.x), (int)e.y);
+    }
   }
   template <class F>
   __device__ __forceinline__ void by_chunk(Lds &L, F f) const {
@@ -315,7 +294,7 @@ struct Found {
 // reaches target, the bin holding more tokens than can be ranked: by the bits
 // of the logit, then by index.  before: the sum in front of the bin.
 template <bool MASS, class S>
-__device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, Row &R, const Found &F) {
+__device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Tokens &row, Row &R, const Found &F) {
   const int b0 = F.bin;
   u64 rest = F.rest, own = F.own;
   uint32_t hi = 0xffffffffu, lo = 0u;
@@ -386,9 +365,9 @@ __device__ __forceinline__ void cut_wide(Lds &L, const S &src, const Row0 &row, 
 // the present cut, or their weight -- reaches target_of(total).  Logits below
 // zq need not be counted.
 template <bool MASS, class S, class F>
-__device__ __forceinline__ Found find_bin(Lds &L, S &&src, const Row &R, float zq, F target_of) {
+__device__ __forceinline__ Found find_bin(Lds &L, const S &src, const Row &R, float zq, F target_of) {
   clear_bins(L);
-  src.template each<4>([&](float z, int i) {
+  src.each([&](float z, int i) {
     if (!(z < zq) && kept(R, z, i)) atomicAdd(&L.bin[bin_of(R, z)], MASS ? weight(R, z) : 1ull);
   });
   u64 total;
@@ -399,7 +378,7 @@ __device__ __forceinline__ Found find_bin(Lds &L, S &&src, const Row &R, float z
 // Shortens the cut to the token of that bin at which the sum reaches its
 // target.
 template <bool MASS, class S>
-__device__ __forceinline__ void settle(Lds &L, const S &src, const Row0 &row, Row &R, const Found &F) {
+__device__ __forceinline__ void settle(Lds &L, const S &src, const Tokens &row, Row &R, const Found &F) {
   if (F.bin < 0) return;
   const int b0 = F.bin;
   // the bin's tokens (L.n is 0)
@@ -444,14 +423,73 @@ __device__ __forceinline__ u64 top_p_target(float p, u64 total) {
   const u64 target = (u64)ceil((double)fmaxf(p, 0.f) * (double)total);
   return target < 1 ? 1ull : target;
 }
-// F: top-p's bin, where there is no top-k.
-template <class S>
-__device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row &R, const Settings &A, Found F) {
+// The running sum to reach, of the weights that are left.
+__device__ __forceinline__ u64 draw_target(float u, u64 total) {
+  const u64 x = u > 0.f ? (u64)((double)fminf(u, 1.f) * (double)total) : 0;
+  return (x > total - 1 ? total - 1 : x) + 1;
+}
+__device__ __forceinline__ void put(const Settings &A, int i, u64 w, u64 total) {
+  *A.id = i;
+  if (A.prob) *A.prob = (float)((double)w / (double)total);
+}
+
+// The sum over the workgroup of a value that the first of every eight lanes has.
+__device__ __forceinline__ u64 sum_of_eighths(Lds &L, u64 v) {
+  v = wave_sum64((threadIdx.x & 7) == 0 ? v : 0ull);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) L.wave[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return uni(sum16_64(L.wave[threadIdx.x & 15]));
+}
+
+// n <= SG tokens in the list, eight lanes to each: what stands before a token in
+// the order decides whether it is left, what stands before it by index whether
+// it is drawn.
+__device__ __forceinline__ void draw_few(Lds &L, int n, const Row &R, const Settings &A) {
+  const int m = min((int)threadIdx.x >> 3, n - 1), part = threadIdx.x & 7;
+  const bool own = (int)threadIdx.x >> 3 < n;
+  const float z = __uint_as_float(L.list[m].x);
+  const int i = (int)L.list[m].y;
+  u64 w = weight(R, z);
+  if (own && part == 0) L.gw[m] = w;
+  __syncthreads();
+  u64 before = 0, rank = 0;
+  for (int j = part; j < n; j += 8) {
+    const uint2 e = L.list[j];
+    const float zj = __uint_as_float(e.x);
+    if (zj > z || (zj == z && (int)e.y < i)) before += L.gw[j], ++rank;
+  }
+  before = sum8_64(before);
+  rank = sum8_64(rank);
+  bool in = own && (A.k == 0 || rank < (u64)A.k);
+  if (A.p < 1.f) {
+    const u64 target = top_p_target(A.p, sum_of_eighths(L, in ? w : 0ull));
+    in = in && before < target;
+  }
+  w = in && w >= A.wmin ? w : 0;
+  const u64 total = sum_of_eighths(L, w);
+  if (own && part == 0) L.gw[m] = w;
+  __syncthreads();
+  u64 run = 0;
+  for (int j = part; j < n; j += 8)
+    if ((int)L.list[j].y < i) run += L.gw[j];
+  run = sum8_64(run);
+  const u64 target = draw_target(A.u, total);
+  if (own && part == 0 && run < target && target <= run + w) put(A, i, w, total);
+}
+
+// The cuts of top-k and top-p, and their tokens' sums, from src.  F: top-p's
+// bin, where there is no top-k; border: a source of that bin's tokens.
+template <class S, class B>
+__device__ __forceinline__ void draw(Lds &L, const S &src, const B &border, const Tokens &row, Row &R, const Settings &A,
+                                     Found F) {
   if (A.k) {
     settle<false>(L, src, row, R, find_bin<false>(L, src, R, A.zq, [&](u64) { return (u64)A.k; }));
-    if (A.p < 1.f) F = find_bin<true>(L, src, R, -INFINITY, [&](u64 total) { return top_p_target(A.p, total); });
+    if (A.p < 1.f)
+      settle<true>(L, src, row, R, find_bin<true>(L, src, R, -INFINITY, [&](u64 total) { return top_p_target(A.p, total); }));
+  } else if (A.p < 1.f) {
+    settle<true>(L, border, row, R, F);
   }
-  if (A.p < 1.f) settle<true>(L, src, row, R, F);
   auto left = [&](float z, int i) -> u64 {
     if (z < A.zp || !kept(R, z, i)) return 0;
     const u64 w = weight(R, z);
@@ -461,12 +499,7 @@ __device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row 
   src.by_chunk(L, left);
   // the chunk in which the running sum passes u of the total
   u64 total;
-  const u64 target = scan_find(L,
-                               [&](u64 total) {
-                                 const u64 x = A.u > 0.f ? (u64)((double)fminf(A.u, 1.f) * (double)total) : 0;
-                                 return (x > total - 1 ? total - 1 : x) + 1;
-                               },
-                               total);
+  const u64 target = scan_find(L, [&](u64 all) { return draw_target(A.u, all); }, total);
   const int c = uni(L.at);
   if (c < row.c0 || c >= row.c1) return;
   const float4 v = row.load(c);
@@ -476,48 +509,94 @@ __device__ __forceinline__ void draw(Lds &L, const S &src, const Row0 &row, Row 
   u64 run = L.before + wave_incl(sum) - sum;
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (run < target && target <= run + w[e]) {
-      *A.id = i + e;
-      if (A.prob) *A.prob = (float)((double)w[e] / (double)total);
-    }
+    if (run < target && target <= run + w[e]) put(A, i + e, w[e], total);
     run += w[e];
   }
 }
 
-// NJ: chunks of a wave that the passes over the whole row take from registers
-// (0: they read them again).
-template <int NJ>
+// The row's tokens from zl on (BOUNDED: up to zh) into the list, in no order,
+// from the groups of chunks whose maximum is at least zl.  L.ln: their number, or
+// any above SL where the list has no room for them.
+template <bool BOUNDED>
+__device__ __forceinline__ void list_tokens(Lds &L, const Tokens &row, float zl, float zh) {
+  const int lane = threadIdx.x & 63, groups = (row.c1 - row.c0 + 3) / 4;  // at most 32
+  __syncthreads();
+  if (threadIdx.x == 0) L.ln = 0;
+  __syncthreads();
+  u64 todo = __ballot(lane < groups && L.top[min(row.g0 + lane, SB / 4 - 1)] >= zl);
+  float4 next[4];
+  auto fetch = [&](u64 which) {
+    const int c = row.c0 + 4 * (which ? __builtin_ctzll(which) : 0);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) next[j] = row.load(min(c + j, row.c1 - 1));
+  };
+  if (todo) fetch(todo);
+  while (todo) {
+    const int c0 = row.c0 + 4 * __builtin_ctzll(todo);
+    float4 w[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = next[j];
+    todo &= todo - 1;
+    if (todo) fetch(todo);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (c0 + j >= row.c1) break;
+      const float z[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+      auto listed = [&](int e) { return z[e] >= zl && (!BOUNDED || z[e] <= zh); };
+      u64 hit[4];  // the lanes whose token is listed
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hit[e] = __ballot(listed(e));
+      if ((hit[0] | hit[1] | hit[2] | hit[3]) == 0) continue;
+      const int n = __popcll(hit[0]) + __popcll(hit[1]) + __popcll(hit[2]) + __popcll(hit[3]);
+      int m = 0;  // places in the list, taken at once
+      if (lane == 0) m = atomicAdd(&L.ln, n);
+      m = uni(m);
+      if (m + n > SL) return;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (listed(e)) {
+          const int at = __builtin_amdgcn_mbcnt_hi((uint32_t)(hit[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)hit[e], m));
+          L.list[at] = make_uint2(__float_as_uint(z[e]), (uint32_t)(256 * (c0 + j) + 4 * lane + e));
+        }
+        m += __popcll(hit[e]);
+      }
+    }
+  }
+}
+
 __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   __shared__ Lds L;
   const int r = blockIdx.x, t = threadIdx.x, wv = uni(t >> 6);
   const int chunks = (A.vocab + 255) / 256, per = (chunks + SW - 1) / SW;
-  const Row0 row{A.logits + (size_t)r * A.vocab, A.vocab, min(wv * per, chunks), min((wv + 1) * per, chunks)};
-  Held<NJ ? NJ : 1> held;
-  float zt = -INFINITY;  // this thread's maximum
-  if constexpr (NJ > 0) {
-    held.fetch(row);
-    held.template each<0>([&](float z, int) { zt = fmaxf(z, zt); });
-  } else {
-    row.chunks<8>([&](int, int, const float4 &w) { zt = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), zt); });
-  }
-  // all of the row, for the passes that need it
-  auto &whole = [&]() -> auto & {
-    if constexpr (NJ > 0) return held;
-    else return row;
-  }();
+  const Tokens row{A.logits + (size_t)r * A.vocab, A.vocab, min(wv * per, chunks), min((wv + 1) * per, chunks),
+                   wv * ((per + 3) / 4)};
+  float zt = -INFINITY, zg = -INFINITY;  // this thread's maximum, and its group's
+  row.chunks<8>([&](int c, int, const float4 &w) {
+    zg = fmaxf(fmaxf(fmaxf(w.x, w.y), fmaxf(w.z, w.w)), zg);
+    if (((c - row.c0) & 3) == 3 || c == row.c1 - 1) {
+      const float z = wave_max(zg);
+      if ((t & 63) == 0) L.top[row.g0 + (c - row.c0) / 4] = z;
+      zt = fmaxf(zg, zt);
+      zg = -INFINITY;
+    }
+  });
   float zv = wave_max(zt);
   if ((t & 63) == 0) L.wv[wv] = zv;
-  if (t == 0) L.id = 0x7fffffff, L.ln = 0;
+  if (t == 0) L.id = 0x7fffffff;
   __syncthreads();
   zv = uni(row16_max(L.wv[t & 15]));
   const float temp = A.temperature ? A.temperature[r] : 1.f, mp = A.min_p ? A.min_p[r] : 0.f;
   if (zv == -INFINITY || !(temp > 0.f) || mp > 1.f) {  // nothing above -inf; greedy; the first token alone is left
-    int at = 0x7fffffff;
-    if (zt == zv && zv != -INFINITY)
-      row.each([&](float z, int i) {
-        if (z == zv) at = min(at, i);
-      });
-    if (at != 0x7fffffff) atomicMin(&L.id, at);
+    for (int c = row.c0; c < row.c1 && zv != -INFINITY; c += 4)
+      if (L.top[row.g0 + (c - row.c0) / 4] == zv) {  // the wave's first group that has it
+        for (int j = 0; j < 4; ++j) {
+          const float4 w = row.load(min(c + j, row.c1 - 1));
+          const int i = 256 * min(c + j, row.c1 - 1) + 4 * (t & 63);
+          const int at = w.x == zv ? i : w.y == zv ? i + 1 : w.z == zv ? i + 2 : w.w == zv ? i + 3 : 0x7fffffff;
+          if (at != 0x7fffffff) atomicMin(&L.id, at);
+        }
+        break;
+      }
     __syncthreads();
     if (t == 0) {
       A.ids[r] = zv == -INFINITY ? 0 : L.id;
@@ -557,40 +636,29 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   // the tokens that can be left: top-p's total takes all of the top k
   Found F{-1, 0, 0};
   float zl = s.p < 1.f ? s.zq : fmaxf(s.zq, s.zp);
-  int last = SB;
-  if (!s.k && s.p < 1.f) {
-    F = find_bin<true>(L, whole, R, -INFINITY, [&](u64 total) { return top_p_target(s.p, total); });
-    last = F.bin;
-    zl = uni(lo_of(R, last));
+  const bool p_alone = !s.k && s.p < 1.f;
+  if (p_alone) {
+    F = find_bin<true>(L, row, R, -INFINITY, [&](u64 total) { return top_p_target(s.p, total); });
+    zl = uni(lo_of(R, F.bin));
   }
   if (zl > -INFINITY) {
-    whole.template fours<6>([&](const float4 &w, int i) {
-      const float z[4] = {w.x, w.y, w.z, w.w};
-      if (!__any(fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3])) >= zl)) return;
-      u64 hit[4];  // the lanes whose token it is
-      int n = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        hit[e] = __ballot(!(z[e] < zl) && kept(R, z[e], i + e) && bin_of(R, z[e]) <= last);
-        n += __popcll(hit[e]);
-      }
-      if (n == 0) return;
-      int m = 0;  // places in the list, taken at once
-      if ((t & 63) == 0) m = atomicAdd(&L.ln, n);
-      m = uni(m);
-      const u64 below = (1ull << (t & 63)) - 1;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int at = m + __popcll(hit[e] & below);
-        if ((hit[e] >> (t & 63) & 1) && at < SL) L.lz[at] = z[e], L.li[at] = i + e;
-        m += __popcll(hit[e]);
-      }
-    });
+    zl = uni(fmaxf(zl, R.zcut));
+    list_tokens<false>(L, row, zl, INFINITY);
     __syncthreads();
-    const int n = uni(L.ln);
-    if (n <= SL) return draw(L, List{&L, n}, row, R, s, F);
+    int n = uni(L.ln);
+    if (n <= SL) {
+      if (!p_alone && n <= SG) return draw_few(L, n, R, s);
+      const List list{&L, n};
+      return draw(L, list, list, row, R, s, F);
+    }
+    if (p_alone) {  // too many: those of top-p's bin alone
+      list_tokens<true>(L, row, zl, uni(hi_of(R, F.bin)));
+      __syncthreads();
+      n = uni(L.ln);
+      if (n <= SL) return draw(L, row, List{&L, n}, row, R, s, F);
+    }
   }
-  draw(L, row, row, R, s, F);
+  draw(L, row, row, row, R, s, F);
 }
 
 }  // namespace
@@ -603,8 +671,7 @@ extern "C" int mllm_sample(int rows, int vocab, const float *logits, const float
   MLLM_CHECK((int64_t)rows * ST < (1ll << 32), "%d rows exceed a launch", rows);
   MLLM_CHECK(logits && u && ids, "null pointer");
   const SampleArgs A{logits, temperature, top_p, min_p, u, top_k, ids, probs, vocab};
-  const auto kern = vocab <= 16 * SW * 256 ? k_sample<16> : k_sample<0>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(ST), 0, reinterpret_cast<hipStream_t>(stream), A);
+  hipLaunchKernelGGL(k_sample, dim3((unsigned)rows), dim3(ST), 0, reinterpret_cast<hipStream_t>(stream), A);
   MLLM_HIP(hipGetLastError());
   return 0;
 }
