@@ -291,6 +291,14 @@ int mllm_forward_decode(mllm_model *model, int32_t id, float *logits, int32_t *a
 int mllm_forward_verify(mllm_model *model, const int32_t *ids, int n, int32_t *argmax, float *logits);
 int mllm_max_pass_tokens(const mllm_model *model);
 
+/* No reference counterpart (its engines choose greedily): a token drawn from
+ * the last row of logits that the last mllm_forward_prompt, _decode or _verify
+ * call formed, as mllm_sample draws it, without copying the logits to the
+ * host (those calls may be given logits = NULL).  prob is nullable.  May be
+ * repeated; MLLM_ERR_INVALID after a chain or before the first such call. */
+int mllm_draw(mllm_model *model, float temperature, int32_t top_k, float top_p, float min_p, float u, int32_t *id,
+              float *prob);
+
 /* Chained greedy decode on the device (CHAIN_TOK, webgpu-metal.js:609-610;
  * webgpu.js:1202-1226): starting from token `first` at position cacheLen,
  * run up to n_steps decode steps where each step's argmax feeds the next

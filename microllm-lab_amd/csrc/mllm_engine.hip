@@ -2896,6 +2896,8 @@ struct mllm_model {
   std::vector<Named> tensors;
   float *d_rope_cos = nullptr, *d_rope_sin = nullptr;
   float *d_logits = nullptr;
+  int logits_row = -1;     // the last token's row of d_logits; -1: the last call left none
+  uint32_t *d_draw = nullptr;  // mllm_draw's id and probability
   int *d_hist = nullptr;
   PassState *d_st = nullptr;
   PassState h_st = {};  // the state that the next pass starts from
@@ -3553,6 +3555,7 @@ int generic_create(mllm_model *M) {
     rc = dev_alloc(M, (void **)&A.attp, sizeof(float) * kGenericTokens * NH * ((c.max_seq_len + kGenericSplit - 1) / kGenericSplit) * kGenericPart);
   if (!rc) rc = dev_alloc(M, (void **)&A.h, sizeof(float) * kGenericTokens * FF);
   if (!rc) rc = dev_alloc(M, (void **)&M->d_logits, sizeof(float) * MAXT * (size_t)V);
+  if (!rc) rc = dev_alloc(M, (void **)&M->d_draw, 2 * sizeof(uint32_t));
   if (!rc) rc = dev_alloc(M, (void **)&A.res, sizeof(int) * MAXT);
   if (!rc) rc = dev_alloc(M, (void **)&A.cur, sizeof(GCursor));
   if (!rc) rc = dev_alloc(M, (void **)&M->d_ids, sizeof(int) * ((size_t)c.max_seq_len + 1));
@@ -3744,6 +3747,7 @@ extern "C" int mllm_model_create(const mllm_config *cfg, const void *payload, ui
   if (!rc) rc = dev_alloc(M, (void **)&P.attpt, sizeof(uint2) * MAXT * NH * P.nsplit_max * APT);
   if (!rc) rc = dev_alloc(M, (void **)&P.cnt, sizeof(unsigned) * MAXT * NH);
   if (!rc) rc = dev_alloc(M, (void **)&M->d_logits, sizeof(float) * MAXT * (size_t)V);
+  if (!rc) rc = dev_alloc(M, (void **)&M->d_draw, 2 * sizeof(uint32_t));
   if (!rc) rc = dev_alloc(M, (void **)&P.amv, sizeof(float) * MAXT * P.lm_tiles);
   if (!rc) rc = dev_alloc(M, (void **)&P.ami, sizeof(int) * MAXT * P.lm_tiles);
   if (!rc) rc = dev_alloc(M, (void **)&P.amt, sizeof(uint2) * 4 * P.lm_tiles);
@@ -4183,12 +4187,14 @@ extern "C" int mllm_forward_prompt(mllm_model *M, const int32_t *ids, int n, flo
   MLLM_CHECK(M && ids, "null argument");
   MLLM_CHECK(n > 0 && n <= M->cfg.max_seq_len, "prompt length %d out of range", n);
   if (int rc = check_ids(M, ids, n)) return rc;
+  M->logits_row = -1;
   if (M->generic) {
     // batched from 3 tokens on: two token steps of the 135M shape take less
     // than the batch's launches
     const bool batch = M->gp.tc > 0 && n >= 3 && !M->dbg_on;
     if (int rc = batch ? g_prompt(M, ids, n, logits, argmax) : g_run(M, ids, n, 0, false, logits, argmax)) return rc;
     M->cache_len = n;
+    M->logits_row = 0;
     return 0;
   }
   if (M->pf_min > 0 && n >= M->pf_min && !M->dbg_on) {
@@ -4206,6 +4212,7 @@ extern "C" int mllm_forward_prompt(mllm_model *M, const int32_t *ids, int n, flo
     MLLM_HIP(hipEventElapsedTime(&M->last_ms, M->ev_pf, M->ev1));
     M->last_tokens = n;
     M->cache_len = n;
+    M->logits_row = 0;
     if (argmax) memcpy(argmax, M->h_out, sizeof(int32_t));
     if (logits) memcpy(logits, M->h_out + 1, words * 4);
     return 0;
@@ -4214,6 +4221,7 @@ extern "C" int mllm_forward_prompt(mllm_model *M, const int32_t *ids, int n, flo
     const int m = std::min(M->max_pass, n - p0);
     const bool last = p0 + m == n;
     if (int rc = run_pass(M, ids + p0, m, p0, last ? 1 : 0, last ? logits : nullptr, last ? argmax : nullptr)) return rc;
+    M->logits_row = last ? m - 1 : -1;
   }
   M->cache_len = n;
   return 0;
@@ -4223,13 +4231,12 @@ extern "C" int mllm_forward_decode(mllm_model *M, int32_t id, float *logits, int
   MLLM_CHECK(M, "null model");
   MLLM_CHECK(M->cache_len < M->cfg.max_seq_len, "KV cache full (%d)", M->cache_len);
   if (int rc = check_ids(M, &id, 1)) return rc;
-  if (M->generic) {
-    if (int rc = g_run(M, &id, 1, M->cache_len, false, logits, argmax)) return rc;
-    M->cache_len += 1;
-    return 0;
-  }
-  if (int rc = run_pass(M, &id, 1, M->cache_len, 1, logits, argmax)) return rc;
+  M->logits_row = -1;
+  if (int rc = M->generic ? g_run(M, &id, 1, M->cache_len, false, logits, argmax)
+                          : run_pass(M, &id, 1, M->cache_len, 1, logits, argmax))
+    return rc;
   M->cache_len += 1;
+  M->logits_row = 0;
   return 0;
 }
 
@@ -4238,13 +4245,27 @@ extern "C" int mllm_forward_verify(mllm_model *M, const int32_t *ids, int n, int
   MLLM_CHECK(n > 0 && n <= M->max_pass, "verify length %d out of range [1, %d]", n, M->max_pass);
   MLLM_CHECK(M->cache_len + n <= M->cfg.max_seq_len, "verify pass exceeds the context");
   if (int rc = check_ids(M, ids, n)) return rc;
-  if (M->generic) {
-    if (int rc = g_run(M, ids, n, M->cache_len, true, logits, argmax)) return rc;
-    M->cache_len += n;
-    return 0;
-  }
-  if (int rc = run_pass(M, ids, n, M->cache_len, 2, logits, argmax)) return rc;
+  M->logits_row = -1;
+  if (int rc = M->generic ? g_run(M, ids, n, M->cache_len, true, logits, argmax)
+                          : run_pass(M, ids, n, M->cache_len, 2, logits, argmax))
+    return rc;
   M->cache_len += n;
+  M->logits_row = n - 1;
+  return 0;
+}
+
+extern "C" int mllm_draw(mllm_model *M, float temperature, int32_t top_k, float top_p, float min_p, float u, int32_t *id,
+                         float *prob) {
+  MLLM_CHECK(M && id, "null argument");
+  MLLM_CHECK(M->logits_row >= 0, "no logits to draw from: the last call was not a prompt, a decode step or a verify pass");
+  if (int rc = sample_row(M->cfg.vocab_size, M->d_logits + (size_t)M->logits_row * M->cfg.vocab_size, temperature, top_k,
+                          top_p, min_p, u, reinterpret_cast<int32_t *>(M->d_draw),
+                          reinterpret_cast<float *>(M->d_draw + 1), M->stream))
+    return rc;
+  if (int rc = fetch(M, M->d_draw, 2, nullptr, 0)) return rc;
+  MLLM_HIP(hipStreamSynchronize(M->stream));
+  memcpy(id, M->h_out, sizeof(int32_t));
+  if (prob) memcpy(prob, M->h_out + 1, sizeof(float));
   return 0;
 }
 
@@ -4256,6 +4277,7 @@ extern "C" int mllm_decode_chain(mllm_model *M, int32_t first, int n_steps, int3
   MLLM_CHECK(n_hist >= 0 && n_hist + n_steps <= M->cfg.max_seq_len, "history too long");
   MLLM_CHECK(n_hist == 0 || hist, "null history");
   if (int rc = check_ids(M, &first, 1)) return rc;
+  M->logits_row = -1;
   if (n_hist) MLLM_HIP(hipMemcpyAsync(M->d_hist, hist, sizeof(int32_t) * n_hist, hipMemcpyHostToDevice, M->stream));
   if (M->generic) {
     // each step's argmax lands at d_hist[n_hist + i] and is step i + 1's
@@ -4319,6 +4341,7 @@ extern "C" int mllm_profile_decode(mllm_model *M, int32_t first, int n_steps, fl
   MLLM_CHECK(n_steps > 0, "n_steps %d", n_steps);
   MLLM_CHECK(M->cache_len + n_steps <= M->cfg.max_seq_len, "profile run exceeds the context");
   if (int rc = check_ids(M, &first, 1)) return rc;
+  M->logits_row = -1;
   const auto phases = pass_phases(M, true, 1);
   const int per_step = (int)phases.size();
   if ((int)M->prof_ev.size() < 2 * per_step) {

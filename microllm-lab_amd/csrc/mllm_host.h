@@ -23,6 +23,11 @@ size_t gemv_q4_argmax_scratch(int m, int n);
 int gemv_q4_argmax_into(int m, int n, const uint8_t *packed, const float *scale, const float *x, float *y,
                         int32_t *argmax, unsigned char *scratch, hipStream_t st);
 
+// mllm_sample for one row with settings in host memory; id and prob are device
+// pointers.
+int sample_row(int vocab, const float *logits, float temperature, int32_t top_k, float top_p, float min_p, float u,
+               int32_t *id, float *prob, hipStream_t st);
+
 }  // namespace mllm
 
 #define MLLM_HIP(expr)                                                   \

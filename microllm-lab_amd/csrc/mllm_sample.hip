@@ -50,6 +50,9 @@ struct SampleArgs {
   int32_t *ids;
   float *probs;
   int vocab;
+  // every row's, where the array is null
+  float temperature1, top_p1, min_p1, u1;
+  int32_t top_k1;
 };
 
 // Order-preserving bits of a float (-0 and +0 tie, as the numbers do).
@@ -585,7 +588,7 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   if (t == 0) L.id = 0x7fffffff;
   __syncthreads();
   zv = uni(row16_max(L.wv[t & 15]));
-  const float temp = A.temperature ? A.temperature[r] : 1.f, mp = A.min_p ? A.min_p[r] : 0.f;
+  const float temp = A.temperature ? A.temperature[r] : A.temperature1, mp = A.min_p ? A.min_p[r] : A.min_p1;
   if (zv == -INFINITY || !(temp > 0.f) || mp > 1.f) {  // nothing above -inf; greedy; the first token alone is left
     for (int c = row.c0; c < row.c1 && zv != -INFINITY; c += 4)
       if (L.top[row.g0 + (c - row.c0) / 4] == zv) {  // the wave's first group that has it
@@ -617,10 +620,10 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   R.icut = 0x7fffffff;
   Settings s;
   s.id = A.ids + r, s.prob = A.probs ? A.probs + r : nullptr;
-  s.u = A.u[r];
-  s.k = A.top_k ? A.top_k[r] : 0;
+  s.u = A.u ? A.u[r] : A.u1;
+  s.k = A.top_k ? A.top_k[r] : A.top_k1;
   if (s.k < 0 || s.k >= A.vocab) s.k = 0;
-  s.p = A.top_p ? A.top_p[r] : 1.f;
+  s.p = A.top_p ? A.top_p[r] : A.top_p1;
   s.wmin = mp > 0.f ? (u64)ceil((double)mp * (double)(1ull << WBITS)) : 0;
   s.zq = s.zp = -INFINITY;
   if (mp > 0.f && zv != INFINITY) s.zp = uni(zv + logf(mp) * temp * 1.00001f - 1e-5f * temp - R.slack);
@@ -661,17 +664,28 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   draw(L, row, row, row, R, s, F);
 }
 
+int launch(int rows, const SampleArgs &A, hipStream_t st) {
+  MLLM_CHECK(rows > 0 && A.vocab > 0, "invalid shape rows=%d vocab=%d", rows, A.vocab);
+  if (A.vocab > kMaxVocab) return set_error(MLLM_ERR_UNSUPPORTED, "vocab=%d exceeds %d", A.vocab, kMaxVocab);
+  MLLM_CHECK((int64_t)rows * ST < (1ll << 32), "%d rows exceed a launch", rows);
+  hipLaunchKernelGGL(k_sample, dim3((unsigned)rows), dim3(ST), 0, st, A);
+  MLLM_HIP(hipGetLastError());
+  return 0;
+}
+
 }  // namespace
+
+int mllm::sample_row(int vocab, const float *logits, float temperature, int32_t top_k, float top_p, float min_p, float u,
+                     int32_t *id, float *prob, hipStream_t st) {
+  const SampleArgs A{logits, nullptr, nullptr, nullptr, nullptr,     nullptr, id,
+                     prob,   vocab,   temperature, top_p, min_p, u, top_k};
+  return launch(1, A, st);
+}
 
 extern "C" int mllm_sample(int rows, int vocab, const float *logits, const float *temperature, const int32_t *top_k,
                            const float *top_p, const float *min_p, const float *u, int32_t *ids, float *probs,
                            void *stream) {
-  MLLM_CHECK(rows > 0 && vocab > 0, "invalid shape rows=%d vocab=%d", rows, vocab);
-  if (vocab > kMaxVocab) return set_error(MLLM_ERR_UNSUPPORTED, "vocab=%d exceeds %d", vocab, kMaxVocab);
-  MLLM_CHECK((int64_t)rows * ST < (1ll << 32), "%d rows exceed a launch", rows);
   MLLM_CHECK(logits && u && ids, "null pointer");
-  const SampleArgs A{logits, temperature, top_p, min_p, u, top_k, ids, probs, vocab};
-  hipLaunchKernelGGL(k_sample, dim3((unsigned)rows), dim3(ST), 0, reinterpret_cast<hipStream_t>(stream), A);
-  MLLM_HIP(hipGetLastError());
-  return 0;
+  const SampleArgs A{logits, temperature, top_p, min_p, u, top_k, ids, probs, vocab, 1.f, 1.f, 0.f, 0.f, 0};
+  return launch(rows, A, reinterpret_cast<hipStream_t>(stream));
 }

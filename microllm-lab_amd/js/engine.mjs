@@ -176,10 +176,28 @@ export class HipPetitGPT {
     return native.lastTiming(this._h);
   }
 
+  /** forwardDecode without the logits' way to the host: for draw(). */
+  decodeStep(id) {
+    native.forwardDecode(this._h, id, null);
+  }
+
   /**
-   * Greedy generation.  mode: "greedy" (host loop, infer.js:603-646),
-   * "chain" (device-chained, webgpu.js:1202-1226) or "spec" (prompt-lookup
-   * speculation, webgpu.js:1239-1270; llama models).
+   * {id, prob}: a token drawn on the device from the last call's last row of
+   * logits with the random number u of [0, 1) (mllm_draw); no reference
+   * counterpart.
+   */
+  draw(u, opts) {
+    const o = opts || {};
+    const or = (v, d) => (v !== undefined ? v : d);
+    return native.draw(this._h, or(o.temperature, 1), or(o.topK, 0), or(o.topP, 1), or(o.minP, 0), u);
+  }
+
+  /**
+   * Generation.  mode: "greedy" (host loop, infer.js:603-646), "chain"
+   * (device-chained, webgpu.js:1202-1226), "spec" (prompt-lookup speculation,
+   * webgpu.js:1239-1270; llama models) or "sample" (draw() with the options
+   * temperature, topK, topP, minP and random, a function of numbers of [0, 1),
+   * Math.random if it is not given).
    */
   async generate(inIds, opts) {
     const o = opts || {};
@@ -200,7 +218,10 @@ export class HipPetitGPT {
     const logits = this.forwardPrompt(ids);
     const ttft = now() - t0;
     const out = [];
-    let next = this.isGpt2 ? argmaxGpt2(logits, []) : this.lastArgmax;
+    const random = o.random || Math.random;
+    let next;
+    if (mode === "sample") next = this.draw(random(), o).id;
+    else next = this.isGpt2 ? argmaxGpt2(logits, []) : this.lastArgmax;
     out.push(next);
     let specHits = 0;
     let specTries = 0;
@@ -213,6 +234,18 @@ export class HipPetitGPT {
         if (ids.length + out.length >= this.cfg.maxSeqLen) break;
         const step = this.forwardDecode(next);
         next = this.isGpt2 ? argmaxGpt2(step, out) : this.lastArgmax;
+        out.push(next);
+        if (onToken) await onToken(next, { phase: "decode" });
+        if (next === eosId) {
+          stopReason = "eos";
+          break;
+        }
+      }
+    } else if (mode === "sample") {
+      for (let i = 1; i < maxNewTokens; i++) {
+        if (ids.length + out.length >= this.cfg.maxSeqLen) break;
+        this.decodeStep(next);
+        next = this.draw(random(), o).id;
         out.push(next);
         if (onToken) await onToken(next, { phase: "decode" });
         if (next === eosId) {

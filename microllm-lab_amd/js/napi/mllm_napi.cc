@@ -260,6 +260,30 @@ napi_value ForwardDecode(napi_env env, napi_callback_info info) {
   return make_int(env, am);
 }
 
+// draw(h, temperature, topK, topP, minP, u) -> {id, prob}
+napi_value Draw(napi_env env, napi_callback_info info) {
+  napi_value argv[6];
+  if (!get_args(env, info, 6, argv)) return nullptr;
+  Handle *h = get_handle(env, argv[0]);
+  if (!h) return nullptr;
+  double v[6];
+  for (int k = 1; k < 6; ++k)
+    if (napi_get_value_double(env, argv[k], &v[k]) != napi_ok) {
+      napi_throw_type_error(env, nullptr, "draw: numbers expected");
+      return nullptr;
+    }
+  int32_t id = 0;
+  float prob = 0.f;
+  MLLM_OK_OR_THROW("mllm_draw", mllm_draw(h->model, (float)v[1], get_i32(env, argv[2]), (float)v[3], (float)v[4],
+                                          (float)v[5], &id, &prob));
+  napi_value out, p;
+  napi_create_object(env, &out);
+  napi_set_named_property(env, out, "id", make_int(env, id));
+  napi_create_double(env, prob, &p);
+  napi_set_named_property(env, out, "prob", p);
+  return out;
+}
+
 // forwardVerify(h, ids: Int32Array, argmax: Int32Array, logits: Float32Array | null)
 napi_value ForwardVerify(napi_env env, napi_callback_info info) {
   napi_value argv[4];
@@ -392,6 +416,7 @@ napi_value Init(napi_env env, napi_value exports) {
       {"createModel", CreateModel}, {"destroy", Destroy},           {"resetCache", ResetCache},
       {"cacheLen", CacheLen},       {"setCacheLen", SetCacheLen},   {"forwardPrompt", ForwardPrompt},
       {"forwardDecode", ForwardDecode}, {"forwardVerify", ForwardVerify}, {"decodeChain", DecodeChain},
+      {"draw", Draw},
       {"gemv", Gemv},               {"setExecMode", SetExecMode},   {"setPrefill", SetPrefill},   {"lastTiming", LastTiming},
       {"deviceBytes", DeviceBytes}, {"maxPassTokens", MaxPass},     {"version", Version},
       {"setDebug", SetDebug},

@@ -58,6 +58,7 @@ SIGNATURES = {
     "mllm_forward_decode": ([P, C.c_int32, P, P], I),
     "mllm_forward_verify": ([P, P, I, P, P], I),
     "mllm_max_pass_tokens": ([P], I),
+    "mllm_draw": ([P, F, C.c_int32, F, F, F, P, P], I),
     "mllm_decode_chain": ([P, C.c_int32, I, C.c_int32, P, I, P, P], I),
     "mllm_model_gemv": ([P, C.c_char_p, P, P], I),
     "mllm_set_exec_mode": ([P, I], I),

@@ -5,13 +5,15 @@ the same surface: constructor(bundle), forwardPrompt, forwardDecode, generate,
 resetCache, cacheLen, gemv, destroy.  All compute runs in libmllm's HIP
 kernels; there is no CPU fallback.
 
-generate() implements three drivers of the same decode step:
+generate() implements four drivers of the same decode step:
   mode="greedy"  host loop of forwardDecode + argmax (infer.js:603-646)
   mode="chain"   device-chained decode, argmax fed back on the GPU
                  (webgpu.js:1202-1226, CHAIN_TOK)
   mode="spec"    prompt-lookup speculation: draft k tokens with lookupDraft
                  (webgpu.js:846-865) and verify k+1 positions in one pass,
                  greedy acceptance (webgpu.js:1239-1270)
+  mode="sample"  host loop of forwardDecode + draw: temperature, top-k, top-p
+                 and min-p on the device (no reference counterpart)
 """
 from __future__ import annotations
 
@@ -201,6 +203,18 @@ class PetitGPT:
         self.last_argmax = am.value
         return self._logits
 
+    def decodeStep(self, token_id: int):
+        """forwardDecode without the logits' way to the host: for draw()."""
+        abi.call("mllm_forward_decode", self._h, int(token_id), None, None)
+
+    def draw(self, u: float, temperature: float = 1.0, topK: int = 0, topP: float = 1.0, minP: float = 0.0):
+        """(token, probability) drawn from the last call's last row of logits
+        with the random number u of [0, 1) (mllm_draw)."""
+        tok, prob = C.c_int32(0), C.c_float(0)
+        abi.call("mllm_draw", self._h, float(temperature), int(topK), float(topP), float(minP), float(u), C.byref(tok),
+                 C.byref(prob))
+        return tok.value, prob.value
+
     def forwardVerify(self, ids, want_logits: bool = False):
         """The (k+1)-row pass: argmax per row (and optionally [n][V] logits)."""
         a = np.ascontiguousarray(np.asarray(ids, np.int32))
@@ -233,7 +247,10 @@ class PetitGPT:
         return device_argmax
 
     def generate(self, ids, maxNewTokens: int = 64, eosId: int = -1, onToken: Optional[Callable] = None,
-                 mode: str = "greedy", specK: int = 4, ngram: int = 3, chainChunk: int = 64) -> dict:
+                 mode: str = "greedy", specK: int = 4, ngram: int = 3, chainChunk: int = 64,
+                 temperature: float = 1.0, topK: int = 0, topP: float = 1.0, minP: float = 0.0,
+                 random: Optional[Callable[[], float]] = None) -> dict:
+        """random: numbers of [0, 1) for mode "sample" (default: numpy's generator)."""
         c = self.cfg
         max_seq = c.max_seq_len or 2048
         ids = list(ids)
@@ -247,7 +264,12 @@ class PetitGPT:
         logits = self.forwardPrompt(ids)
         ttft = (time.perf_counter() - t0) * 1e3
         out: List[int] = []
-        nxt = argmax_gpt2(logits, []) if self.is_gpt2 else self.last_argmax
+        if mode == "sample":
+            random = random or np.random.default_rng().random
+            settings = dict(temperature=temperature, topK=topK, topP=topP, minP=minP)
+            nxt = self.draw(random(), **settings)[0]
+        else:
+            nxt = argmax_gpt2(logits, []) if self.is_gpt2 else self.last_argmax
         out.append(nxt)
         spec_hits = spec_tries = 0
         stop = "max_new_tokens"
@@ -261,6 +283,18 @@ class PetitGPT:
                     break
                 lg = self.forwardDecode(nxt)
                 nxt = self._pick(lg, out, self.last_argmax)
+                out.append(nxt)
+                if onToken:
+                    onToken(nxt, {"phase": "decode"})
+                if nxt == eosId:
+                    stop = "eos"
+                    break
+        elif mode == "sample":
+            for _ in range(1, maxNewTokens):
+                if len(ids) + len(out) >= c.max_seq_len:
+                    break
+                self.decodeStep(nxt)
+                nxt = self.draw(random(), **settings)[0]
                 out.append(nxt)
                 if onToken:
                     onToken(nxt, {"phase": "decode"})
