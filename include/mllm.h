@@ -144,7 +144,8 @@ int mllm_dequant_q4(int m, int n, const uint8_t *packed, const float *scale, int
  *   page * page_stride + h * head_stride + slot * row_stride + d
  * of k and of v; three zero strides mean [pages][n_kv_heads][page_size][head_dim].
  * Position p of sequence s is slot p % page_size of page table[s][p / page_size].
- * Sequences may share pages.  k, v and the strides are 16-byte aligned. */
+ * Sequences may share pages.  k, v and the strides are 16-byte aligned.  A
+ * sequence has at most 2^30 positions (page_size * table_cols). */
 typedef struct mllm_kv_pages {
   void *k, *v;
   int32_t storage; /* MLLM_F32, MLLM_F16 or MLLM_BF16 */

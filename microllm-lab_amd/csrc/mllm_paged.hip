@@ -157,7 +157,8 @@ int check_pages(const mllm_kv_pages *kv, Pages *out) {
     return set_error(MLLM_ERR_UNSUPPORTED, "storage %d unsupported (f32, f16 or bf16)", kv->storage);
   if (kv->head_dim <= 0 || kv->head_dim % 32 || kv->head_dim > 256)
     return set_error(MLLM_ERR_UNSUPPORTED, "head_dim %d unsupported (a multiple of 32, at most 256)", kv->head_dim);
-  MLLM_CHECK((int64_t)kv->page_size * kv->table_cols < (1ll << 31), "%d pages of %d positions a sequence exceed 2^31",
+  // the kernels step past a position in 32 bits
+  MLLM_CHECK((int64_t)kv->page_size * kv->table_cols <= (1ll << 30), "%d pages of %d positions a sequence exceed 2^30",
              kv->table_cols, kv->page_size);
   int64_t ps = kv->page_stride, hs = kv->head_stride, rs = kv->row_stride;
   if (!ps && !hs && !rs) {
@@ -194,7 +195,7 @@ void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *s
   *chunk = 0;
   for (int64_t s = 1; s <= kParts; ++s) {
     int64_t c = ((max_len + s - 1) / s + 255) / 256 * 256;
-    c = c < 256 ? 256 : c > 0x7fffff00 ? 0x7fffff00 : c;
+    c = c < 256 ? 256 : c;
     const int64_t parts = max_len > c ? (max_len + c - 1) / c : 1;
     const int64_t cost = (units * parts + kCus - 1) / kCus * (c * pos_bytes + kStart) + (parts > 1 ? kJoinCost : 0);
     if (*chunk == 0 || cost < best) best = cost, *chunk = (int)c, *splits = (int)parts;

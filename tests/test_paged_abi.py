@@ -86,3 +86,12 @@ def test_sample_refusals(over, code):
     a.update(over)
     rc = abi.lib().mllm_sample(a["rows"], a["vocab"], a["logits"], None, None, None, None, a["u"], a["ids"], None, None)
     assert rc == code and abi.lib().mllm_last_error()
+
+
+@pytest.mark.parametrize("size,cols", [(1 << 20, 2047), (1 << 20, 1025), ((1 << 30) + 1, 1), (1, (1 << 31) - 1)])
+def test_positions_past_2_to_the_30_are_refused(size, cols):
+    """Positions are stepped past in 32 bits: near 2^31 the steps would wrap."""
+    kv = pages(page_size=size, table_cols=cols)
+    assert rope(kv) == INVALID and attn(kv, max_len=size * cols) == INVALID
+    assert abi.lib().mllm_attn_paged_workspace(kv, 3, 4, size * cols) == 0
+    assert b"2^30" in abi.lib().mllm_last_error()
