@@ -234,8 +234,7 @@ int attn_shape(const mllm_kv_pages *kv, const Pages &P, int rows, int n_heads, i
   pl->tiles = (pl->rep + aq - 1) / aq;
   pl->units = (int64_t)rows * P.n_kv * pl->tiles;
   pl->pos_bytes = 2 * P.hd * (kv->storage == MLLM_F32 ? 4 : 2);
-  MLLM_CHECK(pl->units * 64 * AW < (1ll << 32), "%d rows of %d heads exceed a launch", rows,
-             n_heads);
+  MLLM_CHECK(pl->units < (1ll << 32) / (64 * AW), "%d rows of %d heads exceed a launch", rows, n_heads);
   attn_plan(pl->units, max_len, pl->pos_bytes, &pl->chunk, &pl->splits);
   pl->bytes = pl->splits > 1 ? kCounters * sizeof(unsigned) +
                                    (uint64_t)pl->units * pl->splits * (((uint64_t)pl->heads * (P.hd + 2) + 3) & ~3ull) * sizeof(float)

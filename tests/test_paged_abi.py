@@ -95,3 +95,12 @@ def test_positions_past_2_to_the_30_are_refused(size, cols):
     assert rope(kv) == INVALID and attn(kv, max_len=size * cols) == INVALID
     assert abi.lib().mllm_attn_paged_workspace(kv, 3, 4, size * cols) == 0
     assert b"2^30" in abi.lib().mllm_last_error()
+
+
+def test_the_largest_rows_and_heads_are_refused():
+    """2^62 workgroups: their threads wrap 64 bits."""
+    n = (1 << 31) - 1
+    kv = pages(n_kv_heads=n, head_dim=32, sequences=n)
+    assert abi.lib().mllm_attn_paged_workspace(kv, n, n, 64) == 0
+    assert attn(kv, rows=n, heads=n) == INVALID and b"exceed a launch" in abi.lib().mllm_last_error()
+    assert rope(kv, tokens=n, heads=n) == INVALID
