@@ -192,13 +192,15 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  * Sums and the products with the values are float32; the queries multiply the
  * keys as float32 too, with an f16 cache as two f16 pieces (22 bits).  The
  * workspace is mllm_attn_paged_workspace() bytes, 16-byte aligned (NULL where
- * that is 0).  Its first 16384 bytes are zero before the first call with it;
+ * that is 0); one for the most rows and the longest max_len serves all calls.
+ * Its first 16384 bytes are zero before the first call with it;
  * every call leaves them so, and calls of other shapes may share it.  Calls
  * that may overlap need one each. */
 int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, const float *q, const int32_t *seq,
                     const int32_t *len, int max_len, float scale, float *out, void *workspace,
                     uint64_t workspace_bytes, void *stream);
-/* Its bytes for these arguments (0 also for arguments that the call refuses). */
+/* Its bytes for these arguments, which also serve fewer rows and a smaller
+ * max_len of the same heads (0 also for arguments that the call refuses). */
 uint64_t mllm_attn_paged_workspace(const mllm_kv_pages *kv, int rows, int n_heads, int max_len);
 
 /* ids[r]: a token drawn from each row of logits [rows][vocab] with the random

@@ -189,6 +189,8 @@ hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 // units of 6144 positions, 1 / 2 / 3 / 4 / 6 parts 111 / 98 / 89 / 88 / 99; 100
 // units of 4000, 2 / 3 / 4 / 8 parts 23 / 27 / 24 / 28.
 constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
+// At most kCounters workgroups where rows are split: a workspace for many rows
+// and long ones serves fewer and shorter.
 constexpr int64_t kCus = 256, kStart = 64 << 10, kJoinCost = 96 << 10;
 void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *splits) {
   int64_t best = 0;
@@ -199,7 +201,7 @@ void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *s
     const int64_t parts = max_len > c ? (max_len + c - 1) / c : 1;
     const int64_t cost = (units * parts + kCus - 1) / kCus * (c * pos_bytes + kStart) + (parts > 1 ? kJoinCost : 0);
     if (*chunk == 0 || cost < best) best = cost, *chunk = (int)c, *splits = (int)parts;
-    if (units > kCounters || c == 256) break;
+    if (units * (s + 1) > kCounters || c == 256) break;
   }
 }
 
@@ -218,7 +220,10 @@ constexpr int heads_at_most(int dc) {
 struct AttnPlan {
   int rep, tiles, heads, chunk, splits;
   int64_t units, pos_bytes;  // pos_bytes: a head's key and value
-  uint64_t bytes;            // of the workspace: the counters, then the parts
+  uint64_t part_bytes;
+  // of a workspace: the counters, then the parts
+  uint64_t bytes(int64_t parts) const { return kCounters * sizeof(unsigned) + (uint64_t)parts * part_bytes; }
+  uint64_t need() const { return splits > 1 ? bytes(units * splits) : 0; }
 };
 
 int attn_shape(const mllm_kv_pages *kv, const Pages &P, int rows, int n_heads, int max_len, AttnPlan *pl) {
@@ -236,9 +241,7 @@ int attn_shape(const mllm_kv_pages *kv, const Pages &P, int rows, int n_heads, i
   pl->pos_bytes = 2 * P.hd * (kv->storage == MLLM_F32 ? 4 : 2);
   MLLM_CHECK(pl->units < (1ll << 32) / (64 * AW), "%d rows of %d heads exceed a launch", rows, n_heads);
   attn_plan(pl->units, max_len, pl->pos_bytes, &pl->chunk, &pl->splits);
-  pl->bytes = pl->splits > 1 ? kCounters * sizeof(unsigned) +
-                                   (uint64_t)pl->units * pl->splits * (((uint64_t)pl->heads * (P.hd + 2) + 3) & ~3ull) * sizeof(float)
-                             : 0;
+  pl->part_bytes = (((uint64_t)pl->heads * (P.hd + 2) + 3) & ~3ull) * sizeof(float);
   return 0;
 }
 
@@ -280,7 +283,9 @@ extern "C" uint64_t mllm_attn_paged_workspace(const mllm_kv_pages *kv, int rows,
   Pages P;
   AttnPlan pl;
   if (check_pages(kv, &P) || attn_shape(kv, P, rows, n_heads, max_len, &pl)) return 0;
-  return pl.bytes;
+  // parts of no plan for as many rows or fewer and as long or shorter exceed these
+  const int64_t longest = ((int64_t)max_len + 255) / 256, splits = longest < kParts ? longest : kParts;
+  return splits > 1 ? pl.bytes(pl.units * splits < kCounters ? pl.units * splits : kCounters) : 0;
 }
 
 extern "C" int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, const float *q, const int32_t *seq,
@@ -290,13 +295,14 @@ extern "C" int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, c
   AttnPlan pl;
   if (int rc = check_pages(kv, &A.P)) return rc;
   if (int rc = attn_shape(kv, A.P, rows, n_heads, max_len, &pl)) return rc;
+  MLLM_CHECK(seq || rows <= A.P.sequences, "%d rows without seq, %d sequences", rows, A.P.sequences);
+  const uint64_t need = pl.need();
+  MLLM_CHECK(need == 0 || workspace, "null workspace, %llu bytes needed", (unsigned long long)need);
+  MLLM_CHECK(workspace_bytes >= need, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
+             (unsigned long long)need);
+  MLLM_CHECK(need == 0 || ((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   MLLM_CHECK(q && len && out, "null pointer");
   MLLM_CHECK(((uintptr_t)q & 15) == 0, "q must be 16-byte aligned");
-  MLLM_CHECK(seq || rows <= A.P.sequences, "%d rows without seq, %d sequences", rows, A.P.sequences);
-  MLLM_CHECK(pl.bytes == 0 || workspace, "null workspace, %llu bytes needed", (unsigned long long)pl.bytes);
-  MLLM_CHECK(workspace_bytes >= pl.bytes, "workspace of %llu bytes, %llu needed", (unsigned long long)workspace_bytes,
-             (unsigned long long)pl.bytes);
-  MLLM_CHECK(pl.bytes == 0 || ((uintptr_t)workspace & 15) == 0, "the workspace must be 16-byte aligned");
   A.q = q, A.seq = seq, A.len = len, A.out = out;
   A.count = static_cast<unsigned *>(workspace);
   A.part = reinterpret_cast<float *>(A.count + kCounters);

@@ -104,3 +104,19 @@ def test_the_largest_rows_and_heads_are_refused():
     assert abi.lib().mllm_attn_paged_workspace(kv, n, n, 64) == 0
     assert attn(kv, rows=n, heads=n) == INVALID and b"exceed a launch" in abi.lib().mllm_last_error()
     assert rope(kv, tokens=n, heads=n) == INVALID
+
+
+def test_a_workspace_for_the_largest_call_serves_smaller_ones():
+    """With an empty workspace the call says what it needs: never more than the
+    function gave for as many rows and as long a cache, or more."""
+    kv = pages(page_size=256, table_cols=1024)
+    size = abi.lib().mllm_attn_paged_workspace
+    at = [(r, n) for r in (1, 2, 3, 5, 16, 60, 130, 700, 2100) for n in (0, 256, 257, 1000, 4000, 6100, 9000, 70000, 262144)]
+    needed = {}
+    for r, n in at:
+        rc, msg = attn(kv, rows=r, max_len=n, seq=B, out=None, nbytes=0), abi.lib().mllm_last_error().decode()
+        assert rc == INVALID  # the workspace, or out
+        needed[r, n] = int(msg.split(" bytes, ")[1].split()[0]) if "needed" in msg else 0
+    assert sum(v > 0 for v in needed.values()) > 20
+    for r, n in at:
+        assert size(kv, r, 4, n) >= max(v for (a, b), v in needed.items() if a <= r and b <= n), (r, n)
