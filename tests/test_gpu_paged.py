@@ -523,6 +523,76 @@ def test_captured_step_replays_with_new_lengths():
         assert torch.equal(cap[1], eager[1]) and torch.equal(cap[2], eager[2]) and torch.equal(cap[3], eager[3]), t
 
 
+@gpu
+def test_steps_on_two_streams_at_once():
+    """Steps of two batches, each on its stream with its own workspace, against
+    the same steps one after another."""
+    g = torch.Generator().manual_seed(31)
+    rng = np.random.default_rng(31)
+    heads, kvh, hd, V = 6, 2, 64, 3001
+    lens = ([700, 3, 1500, 64], [900, 1200])
+    freq = (1e4 ** (-torch.arange(32) / 32.0)).float().cuda()
+    dev = lambda a, t: torch.tensor(a, dtype=t, device="cuda")  # noqa: E731
+    batch = []
+    for ls in lens:
+        R = len(ls)
+        pool = Pool(g, kvh, hd, 16, R, 100, "f16", fill=0.5)
+        nb = abi.lib().mllm_attn_paged_workspace(pool.desc(), R, heads, 1600)
+        batch.append(dict(R=R, pool=pool, ln=dev(ls, torch.int32), pos=dev([n - 1 for n in ls], torch.int32),
+                          x=torch.from_numpy(rng.standard_normal((R, (heads + 2 * kvh) * hd)).astype(np.float32)).cuda(),
+                          z=torch.from_numpy(rng.standard_normal((R, V)).astype(np.float32)).cuda(), u=torch.rand(R).cuda(),
+                          ws=torch.zeros(nb, dtype=torch.uint8, device="cuda"),
+                          k=dev([40] * R, torch.int32), tp=torch.full((R,), 0.9, device="cuda")))
+
+    def step(b, st):
+        R = b["R"]
+        q, o = torch.zeros(R, heads * hd, device="cuda"), torch.zeros(R, heads * hd, device="cuda")
+        ids = torch.zeros(R, dtype=torch.int32, device="cuda")
+        kv = b["pool"].desc()
+
+        def go():
+            abi.call("mllm_rope_kv_paged", kv, R, heads, p(b["x"]), None, p(b["pos"]), p(freq), 64, 0, None, None, 0.0, p(q), st)
+            abi.call("mllm_attn_paged", kv, R, heads, p(q), None, p(b["ln"]), 1600, 0.125, p(o), p(b["ws"]), b["ws"].numel(), st)
+            abi.call("mllm_sample", R, V, p(b["z"]), None, p(b["k"]), p(b["tp"]), None, p(b["u"]), p(ids), None, st)
+        return go, (q, o, ids)
+
+    want = []
+    for b in batch:
+        go, out = step(b, None)
+        go()
+        torch.cuda.synchronize()
+        want.append([t.clone() for t in out])
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    runs = [[step(b, st.cuda_stream) for b, st in zip(batch, streams)] for _ in range(8)]
+    torch.cuda.synchronize()
+    for run in runs:
+        for go, _ in run:
+            go()
+    torch.cuda.synchronize()
+    for run in runs:
+        for (_, out), w in zip(run, want):
+            assert all(torch.equal(a, b) for a, b in zip(out, w))
+    assert all(int(b["ws"][:16384].sum()) == 0 for b in batch)
+
+
+@gpu
+def test_attn_a_workspace_for_the_largest_call():
+    """One workspace, sized for the most rows and positions, for every smaller
+    call; the counters at its head stay zero."""
+    g = torch.Generator().manual_seed(32)
+    rng = np.random.default_rng(32)
+    pool = Pool(g, 2, 64, 16, 40, 375, "f16")
+    nb = abi.lib().mllm_attn_paged_workspace(pool.desc(), 40, 8, 6000)
+    ws = torch.zeros(nb, dtype=torch.uint8, device="cuda")
+    for lens in ([6000, 10], [257], [300] * 40, [2000, 0, 5999, 1, 4000, 256]):
+        q = rng.standard_normal((len(lens), 8, 64)).astype(np.float32)
+        assert abi.lib().mllm_attn_paged_workspace(pool.desc(), len(lens), 8, max(lens)) <= nb
+        o = run_attn(pool, q, None, lens, 8, 0.125, ws=ws)
+        ref, tol = ref_attn(q, pool, range(len(lens)), lens, 8, 0.125)
+        assert (np.abs(o - ref) <= tol).all(), lens
+        assert int(ws[:16384].sum()) == 0
+
+
 # ---------------------------------------------------------------- a model's step
 class PagedLlama:
     """A llama bundle's decode step for several sequences, from the operators."""
