@@ -180,6 +180,8 @@ int check_pages(const mllm_kv_pages *kv, Pages *out) {
 
 hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
+constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
+
 // Positions per workgroup (turns of the four waves) and the number of parts for
 // rows of up to max_len positions.  A CU reads at most about 28 GB/s, whatever
 // the number of its workgroups, and the chip 6.2 TB/s: the time goes by the
@@ -188,20 +190,23 @@ hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 // units, 8 / 12 / 16 / 20 / 24 / 32 parts 239 / 174 / 143 / 199 / 168 / 152; 320
 // units of 6144 positions, 1 / 2 / 3 / 4 / 6 parts 111 / 98 / 89 / 88 / 99; 100
 // units of 4000, 2 / 3 / 4 / 8 parts 23 / 27 / 24 / 28.
-constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
+// A part is a multiple of kChunk positions: one row of 700 positions in float32
+// (3 units), parts of 64 / 128 / 256 positions 8.0 / 8.1 / 9.1 us; five rows of
+// 516 in f16 9.7 / 9.1 / 9.2.
 // At most kCounters workgroups where rows are split: a workspace for many rows
 // and long ones serves fewer and shorter.
-constexpr int64_t kCus = 256, kStart = 64 << 10, kJoinCost = 96 << 10;
+constexpr int64_t kChunk = 128, kCus = 256, kStart = 64 << 10, kJoinCost = 96 << 10;
 void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *splits) {
   int64_t best = 0;
   *chunk = 0;
   for (int64_t s = 1; s <= kParts; ++s) {
-    int64_t c = ((max_len + s - 1) / s + 255) / 256 * 256;
-    c = c < 256 ? 256 : c;
+    int64_t c = ((max_len + s - 1) / s + kChunk - 1) / kChunk * kChunk;
+    c = c < kChunk ? kChunk : c;
     const int64_t parts = max_len > c ? (max_len + c - 1) / c : 1;
-    const int64_t cost = (units * parts + kCus - 1) / kCus * (c * pos_bytes + kStart) + (parts > 1 ? kJoinCost : 0);
+    const int64_t cost = (units * parts + kCus - 1) / kCus * ((c < max_len ? c : max_len) * pos_bytes + kStart) +
+                         (parts > 1 ? kJoinCost : 0);
     if (*chunk == 0 || cost < best) best = cost, *chunk = (int)c, *splits = (int)parts;
-    if (units * (s + 1) > kCounters || c == 256) break;
+    if (units * (s + 1) > kCounters || c == kChunk) break;
   }
 }
 
@@ -284,7 +289,7 @@ extern "C" uint64_t mllm_attn_paged_workspace(const mllm_kv_pages *kv, int rows,
   AttnPlan pl;
   if (check_pages(kv, &P) || attn_shape(kv, P, rows, n_heads, max_len, &pl)) return 0;
   // parts of no plan for as many rows or fewer and as long or shorter exceed these
-  const int64_t longest = ((int64_t)max_len + 255) / 256, splits = longest < kParts ? longest : kParts;
+  const int64_t longest = ((int64_t)max_len + kChunk - 1) / kChunk, splits = longest < kParts ? longest : kParts;
   return splits > 1 ? pl.bytes(pl.units * splits < kCounters ? pl.units * splits : kCounters) : 0;
 }
 

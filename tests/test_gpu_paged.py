@@ -280,7 +280,7 @@ def test_attn_many_rows_take_one_part():
     g = torch.Generator().manual_seed(11)
     rng = np.random.default_rng(11)
     pool = Pool(g, 4, 64, 16, 300, 9, "f16")
-    lens = [int(v) for v in rng.integers(0, 140, 300)]  # a part is 256 positions at least
+    lens = [int(v) for v in rng.integers(0, 129, 300)]  # a part is 128 positions at least
     q = rng.standard_normal((300, 8, 64)).astype(np.float32)
     assert abi.lib().mllm_attn_paged_workspace(pool.desc(), 300, 8, max(lens)) == 0
     o = run_attn(pool, q, None, lens, 8, 0.125)
