@@ -49,8 +49,7 @@ __device__ __forceinline__ int page_of(const Pages &P, int pos) {
 }
 
 // ---------------------------------------------------------------- attention over pages
-constexpr int AW = 4;                  // waves of a workgroup
-constexpr int ASUB = 2048;             // positions whose places in the pool are in LDS at a time
+constexpr int APLACES = 512;           // positions whose places in the pool are in LDS at a time, for each wave
 constexpr int kCounters = 4096;        // rows' heads that may be split, each with its counter
 constexpr int kParts = 256;            // parts of a row at most
 constexpr float LOG2E = 1.44269504088896340736f;
@@ -63,6 +62,7 @@ struct AttnArgs {
   unsigned *count;    // [kCounters] parts that are there, zero between calls
   int n_heads, rep, tiles, heads, max_len, chunk, splits;  // heads: query heads of a workgroup at most
   float scale;
+  int waves;          // of a workgroup: four, or one for many short rows (splits = 1)
   int stream;         // loads past the caches
 };
 

@@ -195,9 +195,19 @@ constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
 // 516 in f16 9.7 / 9.1 / 9.2.
 // At most kCounters workgroups where rows are split: a workspace for many rows
 // and long ones serves fewer and shorter.
+// Many short rows (more units than the two workgroups of four waves that a CU
+// holds, of at most kShort bytes each) take a wave to a unit, so that eight of
+// them are at their starts and ends at once.  Four waves / one, us: 640 units of
+// 64 f16 elements, 16 / 128 / 512 / 1024 positions 10.6 / 9.0, 12.0 / 9.1, 20.2
+// / 17.6, 36.1 / 35.3; 320 units 8.7 / 8.7, 8.8 / 8.7, 13.4 / 16.6, 20.3 / 28.3;
+// 2560 units 28.6 / 11.7, 32.9 / 19.3, 65.8 / 66.5, 110 / 126; 2048 units of 128
+// bf16 elements, 25 / 128 / 256 / 512 positions 24.7 / 11.7, 35.5 / 25.5, 61.4
+// / 52.2, 91.0 / 95.4.
+constexpr int64_t kShort = 128 << 10;
 constexpr int64_t kChunk = 128, kCus = 256, kStart = 64 << 10, kJoinCost = 96 << 10;
-void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *splits) {
+void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *waves, int *chunk, int *splits) {
   int64_t best = 0;
+  *waves = units > 2 * kCus && max_len * pos_bytes <= kShort ? 1 : 4;
   *chunk = 0;
   for (int64_t s = 1; s <= kParts; ++s) {
     int64_t c = ((max_len + s - 1) / s + kChunk - 1) / kChunk * kChunk;
@@ -206,7 +216,7 @@ void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *chunk, int *s
     const int64_t cost = (units * parts + kCus - 1) / kCus * ((c < max_len ? c : max_len) * pos_bytes + kStart) +
                          (parts > 1 ? kJoinCost : 0);
     if (*chunk == 0 || cost < best) best = cost, *chunk = (int)c, *splits = (int)parts;
-    if (units * (s + 1) > kCounters || c == kChunk) break;
+    if (*waves == 1 || units * (s + 1) > kCounters || c == kChunk) break;
   }
 }
 
@@ -223,7 +233,7 @@ constexpr int heads_at_most(int dc) {
 }
 
 struct AttnPlan {
-  int rep, tiles, heads, chunk, splits;
+  int rep, tiles, heads, waves, chunk, splits;
   int64_t units, pos_bytes;  // pos_bytes: a head's key and value
   uint64_t part_bytes;
   // of a workspace: the counters, then the parts
@@ -244,8 +254,8 @@ int attn_shape(const mllm_kv_pages *kv, const Pages &P, int rows, int n_heads, i
   pl->tiles = (pl->rep + aq - 1) / aq;
   pl->units = (int64_t)rows * P.n_kv * pl->tiles;
   pl->pos_bytes = 2 * P.hd * (kv->storage == MLLM_F32 ? 4 : 2);
-  MLLM_CHECK(pl->units < (1ll << 32) / (64 * AW), "%d rows of %d heads exceed a launch", rows, n_heads);
-  attn_plan(pl->units, max_len, pl->pos_bytes, &pl->chunk, &pl->splits);
+  MLLM_CHECK(pl->units < (1ll << 32) / 256, "%d rows of %d heads exceed a launch", rows, n_heads);
+  attn_plan(pl->units, max_len, pl->pos_bytes, &pl->waves, &pl->chunk, &pl->splits);
   pl->part_bytes = (((uint64_t)pl->heads * (P.hd + 2) + 3) & ~3ull) * sizeof(float);
   return 0;
 }
@@ -313,6 +323,7 @@ extern "C" int mllm_attn_paged(const mllm_kv_pages *kv, int rows, int n_heads, c
   A.part = reinterpret_cast<float *>(A.count + kCounters);
   A.n_heads = n_heads, A.rep = pl.rep, A.tiles = pl.tiles, A.heads = pl.heads, A.max_len = max_len;
   A.chunk = pl.chunk, A.splits = pl.splits, A.scale = scale;
+  A.waves = pl.waves;
   // what the Infinity Cache cannot hold until the next call is read past the
   // caches (64 rows of 6144 positions, 503 MB: 95 to 88 us; 126 MB that it does
   // hold: 29 to 32)

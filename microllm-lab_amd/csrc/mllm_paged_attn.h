@@ -155,12 +155,23 @@ __device__ __forceinline__ v4f mma32(u32x4 a, u32x4 b, v4f c) {
 // workgroup through the chunk again in float32, where it acts as in the plain
 // formula.
 //
-// What bounds it: the cache's bytes.  Per 64 positions of an f16 head of 64
-// elements, 16 KB, a wave spends 16 + 64 MFMAs (770 cycles) and about 1000 VALU
-// cycles; a CU's share of 7 TB/s is 1440 cycles for them.
-// STREAM: the cache is read past the caches.
-template <class KV, int DC, int RT, bool STREAM>
+// What bounds it: the cache's bytes, at about 28 GB/s to a CU and 6.2 TB/s in
+// all, and for short rows a workgroup's start and end.  Per 64 positions of an
+// f16 head of 64 elements, 16 KB, a wave spends 16 + 64 MFMAs (770 cycles) and
+// about 1000 VALU cycles; a SIMD's share of the CU's 28 GB/s is 5600 cycles for
+// them.  Measured, us: 2 rows of 100000 positions, 8 heads of 128 bf16 elements
+// (819 MB), 143 (5.7 TB/s); 64 rows of 512 to 2048, 5 heads of 64 f16 elements
+// (102 MB), 28.8, in which a workgroup takes 1.0 to its row's length, 1.4 to its
+// pages, 2.4 to its first scores, 0.8 for the sums of the lanes and waves, 0.8
+// to store them and 1.7 to join them.  Tried there without gain: three
+// workgroups to a CU in place of two (fewer positions in flight), pages looked
+// up a block ahead (its barriers in the loop cost more than the stops it saves),
+// finer parts under the same two workgroups (33 to 40).
+// STREAM: the cache is read past the caches.  AW: waves of a workgroup; with one
+// there is no joining.
+template <class KV, int DC, int RT, bool STREAM, int AW>
 __global__ __launch_bounds__(64 * AW) void k_attn_paged(AttnArgs A) {
+  constexpr int ASUB = APLACES * AW;  // positions whose places in the pool are in LDS at a time
   using Y = Lay<KV, DC>;
   constexpr int HD = Y::HD, EL = Y::EL, RUN = Y::RUN, NR = Y::NR, LPR = Y::LPR, G = Y::G, PT = Y::PT, TP = Y::TP,
                 NU = Y::NU, PS = Y::PS, NP = Piece<KV>::NP;
@@ -168,7 +179,7 @@ __global__ __launch_bounds__(64 * AW) void k_attn_paged(AttnArgs A) {
   using T = typename KV::T;
   // the places of the positions and the waves' weights; then the waves' sums
   constexpr int kPlaces = 2 * ASUB, kWeights = AW * 4 * RT * PS, kSums = AW * 4 * HD;
-  constexpr int kJoin = 17 * kParts;  // a join's weights and the heads' sums
+  constexpr int kJoin = AW == 1 ? 0 : 17 * kParts;  // a join's weights and the heads' sums
   constexpr int kMain = kPlaces + kWeights > kSums ? kPlaces + kWeights : kSums, kLds = kMain > kJoin ? kMain : kJoin;
   __shared__ __attribute__((aligned(16))) float lds[kLds];
   __shared__ float ml[2][AW][16];
@@ -416,7 +427,8 @@ __global__ __launch_bounds__(64 * AW) void k_attn_paged(AttnArgs A) {
       }
     }
   }
-  if (A.splits == 1) return;
+  if (AW == 1 || A.splits == 1) return;
+  if constexpr (AW > 1) {
   // the last part to be there joins them
   const int parts = n == 0 ? 1 : (n + A.chunk - 1) / A.chunk;
   wait_stores();
@@ -487,16 +499,24 @@ __global__ __launch_bounds__(64 * AW) void k_attn_paged(AttnArgs A) {
     for (int k = 0; k < 4; ++k) to[k] = n == 0 && !bad ? 0.f : oo[k] / ll;
   }
   if (threadIdx.x == 0) __hip_atomic_store(A.count + blockIdx.x, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
 }
 
 // ---------------------------------------------------------------- launch
 template <class KV, int DC>
 int attn_launch(const AttnArgs &A, dim3 grid, hipStream_t st) {
   constexpr int RT4 = Lay<KV, DC>::AQ > 8 ? 4 : 2;
-  const auto kern = A.heads <= 4   ? (A.stream ? k_attn_paged<KV, DC, 1, true> : k_attn_paged<KV, DC, 1, false>)
-                    : A.heads <= 8 ? (A.stream ? k_attn_paged<KV, DC, 2, true> : k_attn_paged<KV, DC, 2, false>)
-                                   : (A.stream ? k_attn_paged<KV, DC, RT4, true> : k_attn_paged<KV, DC, RT4, false>);
-  hipLaunchKernelGGL(kern, grid, dim3(64 * AW), 0, st, A);
+  const auto pick = [&](auto stream, auto waves) {
+    constexpr bool S = decltype(stream)::value;
+    constexpr int W = decltype(waves)::value;
+    const auto kern = A.heads <= 4   ? k_attn_paged<KV, DC, 1, S, W>
+                      : A.heads <= 8 ? k_attn_paged<KV, DC, 2, S, W>
+                                     : k_attn_paged<KV, DC, RT4, S, W>;
+    hipLaunchKernelGGL(kern, grid, dim3(64 * W), 0, st, A);
+  };
+  if (A.waves == 1) pick(std::false_type{}, std::integral_constant<int, 1>{});
+  else if (A.stream) pick(std::true_type{}, std::integral_constant<int, 4>{});
+  else pick(std::false_type{}, std::integral_constant<int, 4>{});
   MLLM_HIP(hipGetLastError());
   return 0;
 }

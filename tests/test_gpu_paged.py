@@ -292,6 +292,62 @@ def test_attn_many_rows_take_one_part():
 
 
 @gpu
+@pytest.mark.parametrize("rows,heads,kvh,hd,storage,page,top", [
+    (300, 6, 2, 64, "f16", 16, 512), (200, 24, 3, 64, "bf16", 7, 200), (180, 3, 3, 128, "bf16", 16, 256),
+    (530, 12, 1, 64, "f32", 24, 90), (300, 4, 2, 32, "f16", 1, 600), (180, 3, 3, 256, "f32", 16, 64)])
+def test_attn_many_short_rows(rows, heads, kvh, hd, storage, page, top):
+    """More units than workgroups of four waves fit the chip, each short: a wave
+    to a unit; with empty rows, padding, a bad page and a length too long."""
+    g = torch.Generator().manual_seed(33)
+    rng = np.random.default_rng(33)
+    seqs = 40
+    pool = Pool(g, kvh, hd, page, seqs, -(-top // page), storage)
+    seq = [int(v) for v in rng.integers(0, seqs, rows)]
+    lens = [int(v) for v in rng.integers(0, top + 1, rows)]
+    lens[:6] = [0, 1, top, top - 1, 2, top]
+    seq[:6] = range(6)
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    kept = [r for r in range(rows) if r not in (7, 9, 11)]
+    seq[7], seq[9] = -1, seqs  # padding
+    table = pool.table.clone()
+    bad = seqs - 1
+    for r in range(rows):
+        if seq[r] == bad:
+            seq[r] = 0
+    seq[11], lens[11] = bad, 1
+    table[bad, 0] = pool.k.shape[0]
+    out = torch.full((rows, heads * hd), 7.0, device="cuda")
+    o = run_attn(pool, q, seq, lens, heads, 0.125, max_len=top, out=out, table=table)
+    assert (o[[7, 9]] == 7.0).all() and np.isnan(o[11]).all() and (o[0] == 0).all()
+    some = kept[:12] + kept[12::17]
+    ref, tol = ref_attn(q[some], pool, [seq[r] for r in some], [lens[r] for r in some], heads, 0.125)
+    assert (np.abs(o[some] - ref) <= tol).all()
+
+
+@gpu
+@pytest.mark.parametrize("storage", ["f32", "f16", "bf16"])
+def test_attn_infinities_in_many_short_rows(storage):
+    """What an infinite key or value does to a row, it does to it in a large batch."""
+    g = torch.Generator().manual_seed(34)
+    rng = np.random.default_rng(34)
+    pool = Pool(g, 2, 64, 16, 6, 8, storage)
+    t = pool.table.long()
+    pool.k[t[1, 0], 0, 3, 5] = float("inf")
+    pool.k[t[2, 1], 1, 0, 7] = float("-inf")
+    pool.v[t[3, 2], 1, 1, 9] = float("inf")
+    pool.k[t[4, 0], 0, 0] = float("nan")
+    q = rng.standard_normal((300, 6, 64)).astype(np.float32)
+    seq = [r % 6 for r in range(300)]
+    lens = [int(v) for v in rng.integers(40, 129, 300)]
+    many = run_attn(pool, q, seq, lens, 6, 0.125, max_len=128)
+    few = np.concatenate([run_attn(pool, q[r:r + 12], seq[r:r + 12], lens[r:r + 12], 6, 0.125, max_len=128)
+                          for r in range(0, 60, 12)])
+    assert np.array_equal(np.isnan(many[:60]), np.isnan(few)) and np.isnan(few).any() and np.isinf(few).any()
+    with np.errstate(invalid="ignore"):  # each is within 2^-17 of the formula
+        assert (np.isclose(many[:60], few, rtol=2.0 ** -16, atol=2.0 ** -16) | np.isnan(few)).all()
+
+
+@gpu
 @pytest.mark.parametrize("scale", [0.125, 3.0, 0.0, -1.0])
 def test_attn_peaked_and_flat_scores(scale):
     g = torch.Generator().manual_seed(12)
