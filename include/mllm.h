@@ -166,7 +166,7 @@ typedef struct mllm_kv_pages {
  *     (2i, 2i + 1) where interleaved != 0, by the angle pos * inv_freq[i],
  *     i < rot / 2, formed in double.  A context scaled for more positions is a
  *     matter of inv_freq.  rot = 0 rotates nothing (inv_freq may be NULL).
- *   - q receives [tokens][n_heads head_dim]; keys and values go to the token's
+ *   - q (like qkv 16-byte aligned) receives [tokens][n_heads head_dim]; keys and values go to the token's
  *     slot, rounded to nearest even (f16: beyond 65504 to infinity).
  * A token whose sequence is outside [0, sequences), or whose position is
  * negative, is padding: nothing is written for it.  One whose position has no
@@ -181,8 +181,8 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  * (n_heads a multiple of n_kv_heads), and row r attends to positions 0 ..
  * len[r] - 1 of sequence seq[r] (seq NULL: sequence r).  Several rows may have
  * one sequence: a speculation pass is a row per token, each one longer.
- * q is 16-byte aligned.  max_len bounds every len (at most page_size * table_cols); the work is split
- * over it, so a host passes the longest it knows of.
+ * q is 16-byte aligned.  max_len bounds every len (at most page_size *
+ * table_cols); the work is split over it, so a host passes the longest it knows of.
  *   - len[r] = 0: out[r] is 0.  A sequence outside [0, sequences) is padding:
  *     out[r] is left as it was.
  *   - len[r] < 0 or > max_len, or a page within the length outside [0, pages):

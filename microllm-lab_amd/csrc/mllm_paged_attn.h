@@ -166,7 +166,8 @@ __device__ __forceinline__ v4f mma32(u32x4 a, u32x4 b, v4f c) {
 // to store them and 1.7 to join them.  Tried there without gain: three
 // workgroups to a CU in place of two (fewer positions in flight), pages looked
 // up a block ahead (its barriers in the loop cost more than the stops it saves),
-// finer parts under the same two workgroups (33 to 40).
+// finer parts under the same two workgroups (33 to 40), parts of one wave each
+// (29.5 to 37).
 // STREAM: the cache is read past the caches.  AW: waves of a workgroup; with one
 // there is no joining.
 template <class KV, int DC, int RT, bool STREAM, int AW>
@@ -514,6 +515,7 @@ int attn_launch(const AttnArgs &A, dim3 grid, hipStream_t st) {
                                      : k_attn_paged<KV, DC, RT4, S, W>;
     hipLaunchKernelGGL(kern, grid, dim3(64 * W), 0, st, A);
   };
+  // a wave to a unit: short rows, through the caches
   if (A.waves == 1) pick(std::false_type{}, std::integral_constant<int, 1>{});
   else if (A.stream) pick(std::true_type{}, std::integral_constant<int, 4>{});
   else pick(std::false_type{}, std::integral_constant<int, 4>{});
