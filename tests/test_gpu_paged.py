@@ -343,8 +343,10 @@ def test_attn_infinities_in_many_short_rows(storage):
     few = np.concatenate([run_attn(pool, q[r:r + 12], seq[r:r + 12], lens[r:r + 12], 6, 0.125, max_len=128)
                           for r in range(0, 60, 12)])
     assert np.array_equal(np.isnan(many[:60]), np.isnan(few)) and np.isnan(few).any() and np.isinf(few).any()
-    with np.errstate(invalid="ignore"):  # each is within 2^-17 of the formula
-        assert (np.isclose(many[:60], few, rtol=2.0 ** -16, atol=2.0 ** -16) | np.isnan(few)).all()
+    with np.errstate(invalid="ignore"):
+        # ref_attn's bound for each: a walk of 4 sqrt(64) max|score| (8) + 4 sqrt(128) + 32 and some, below 350
+        # roundings of 2^-24, times at most max|v| (4.5); two of them are below 2^-12
+        assert (np.isclose(many[:60], few, rtol=0, atol=2.0 ** -12) | np.isnan(few)).all()
 
 
 @gpu
