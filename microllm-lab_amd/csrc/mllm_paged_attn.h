@@ -16,9 +16,9 @@ using namespace mllm::paged;
 // A row's length as the kernels use it: -1 padding (the row is left as it
 // was), -2 not possible (NaN).
 __device__ __forceinline__ int row_len(const AttnArgs &A, int row, int &seq) {
+  const int n = A.len[row];  // both loads in flight
   seq = A.seq ? A.seq[row] : row;
   if (seq < 0 || seq >= A.P.sequences) return -1;
-  const int n = A.len[row];
   return n < 0 || n > A.max_len ? -2 : n;
 }
 
