@@ -266,22 +266,14 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-_abi = None
-
-
 def _library():
-    """The binding, imported once, as a program does."""
-    global _abi
-    if _abi is not None:
-        return _abi
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     at = os.path.join(root, "microllm-lab_amd")
     if at not in sys.path:
         sys.path.insert(0, at)
     from mllm import abi
 
-    _abi = abi
-    return _abi
+    return abi
 
 
 def _handle(abi, s):
