@@ -169,7 +169,8 @@ typedef struct mllm_kv_pages {
  *   - q (like qkv 16-byte aligned) receives [tokens][n_heads head_dim]; keys and values go to the token's
  *     slot, rounded to nearest even (f16: beyond 65504 to infinity).
  * A token whose sequence is outside [0, sequences), or whose position is
- * negative, is padding: nothing is written for it.  One whose position has no
+ * negative, is padding: nothing is written for it.  Its rows of qkv, seq and
+ * pos are read all the same, whatever they hold.  One whose position has no
  * page -- beyond the table, or the table's entry outside [0, pages) -- writes q
  * alone.  Two tokens of one call must not share a slot. */
 int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const float *qkv, const int32_t *seq,
@@ -184,7 +185,8 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  * q is 16-byte aligned.  max_len bounds every len (at most page_size *
  * table_cols); the work is split over it, so a host passes the longest it knows of.
  *   - len[r] = 0: out[r] is 0.  A sequence outside [0, sequences) is padding:
- *     out[r] is left as it was.
+ *     out[r] is left as it was.  Its rows of q, seq and len are read all the
+ *     same, whatever they hold.
  *   - len[r] < 0 or > max_len, or a page within the length outside [0, pages):
  *     out[r] (the heads' rows) is NaN.
  *   - Only positions below len[r] count, whatever the slots behind them hold.
