@@ -623,10 +623,13 @@ __global__ __launch_bounds__(ST) void k_sample(SampleArgs A) {
   R.dmax = (double)fminf(zv, 3.402823466e38f);
   R.c = uni(1.4426950408889634074 / (double)temp);
   R.slack = uni(fabsf(zv) * 2.4e-7f);
-  float dlim = fminf((float)((double)WBITS / R.c), 3.402823466e38f);
+  const double far = (double)WBITS / R.c;
+  float dlim = fminf((float)far, 3.402823466e38f);
   if (dlim < 1e-35f) dlim = 0.f;  // a temperature below 2e-37: the tokens that tie at the maximum
   R.s0 = uni(dlim > 0.f ? (float)SB / dlim : 0.f);
-  R.zcut = uni(fmaxf(zv - dlim, -3.402823466e38f));
+  // from a temperature of 1.1e37 on, logits further apart than the largest float have weight
+  const float zfar = dlim < 3.402823466e38f || zv == INFINITY ? zv - dlim : (float)fmax((double)zv - far, -3.402823466e38);
+  R.zcut = uni(fmaxf(zfar, -3.402823466e38f));
   R.icut = 0x7fffffff;
   Settings s;
   s.id = A.ids + r, s.prob = A.probs ? A.probs + r : nullptr;

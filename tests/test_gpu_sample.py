@@ -200,3 +200,21 @@ def test_sample_frequencies():
     w /= w.sum()
     got = np.bincount(ids, minlength=5) / n
     assert (np.abs(got - w) <= 6 * np.sqrt(w * (1 - w) / n)).all()
+
+
+@gpu
+@pytest.mark.parametrize("temp", [1e37, 1.2e37, 1e38, 3e38, np.inf])
+def test_sample_logits_further_apart_than_the_largest_float(temp):
+    """At temperatures near the largest float, finite logits of both ends of
+    the type weigh what the formula says; +inf still takes all, -inf nothing."""
+    rng = np.random.default_rng(9)
+    R, V = 24, 2003
+    z = (3.2e38 * rng.uniform(-1, 1, (R, V))).astype(np.float32)
+    z[:, 5], z[:, 77] = 3.3e38, -np.finfo(np.float32).max
+    z[R - 1, 9] = np.inf
+    z[R - 2, 100:] = -np.inf
+    u = rng.random(R).astype(np.float32)
+    check(z, temp=temp, u=u)
+    check(z, temp=temp, k=rng.integers(1, V, R), u=u)
+    check(z, temp=temp, top_p=rng.uniform(0.3, 1.0, R), u=u)
+    check(z, temp=temp, min_p=rng.uniform(0.0, 0.05, R), u=u)
