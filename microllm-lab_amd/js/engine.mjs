@@ -176,6 +176,11 @@ export class HipPetitGPT {
     return native.lastTiming(this._h);
   }
 
+  /** forwardPrompt without the logits' way to the host: for draw(). */
+  promptStep(ids) {
+    native.forwardPrompt(this._h, Int32Array.from(ids), null);
+  }
+
   /** forwardDecode without the logits' way to the host: for draw(). */
   decodeStep(id) {
     native.forwardDecode(this._h, id, null);
@@ -215,7 +220,7 @@ export class HipPetitGPT {
     if (mode === "spec" && this.isGpt2) throw new Error("speculative decode needs a llama-style model");
     this.resetCache();
     const t0 = now();
-    const logits = this.forwardPrompt(ids);
+    const logits = mode === "sample" ? this.promptStep(ids) : this.forwardPrompt(ids);
     const ttft = now() - t0;
     const out = [];
     const random = o.random || Math.random;

@@ -203,6 +203,11 @@ class PetitGPT:
         self.last_argmax = am.value
         return self._logits
 
+    def promptStep(self, ids):
+        """forwardPrompt without the logits' way to the host: for draw()."""
+        a = np.ascontiguousarray(np.asarray(ids, np.int32))
+        abi.call("mllm_forward_prompt", self._h, a.ctypes.data, a.size, None, None)
+
     def decodeStep(self, token_id: int):
         """forwardDecode without the logits' way to the host: for draw()."""
         abi.call("mllm_forward_decode", self._h, int(token_id), None, None)
@@ -261,7 +266,7 @@ class PetitGPT:
             raise ValueError("speculative decode is a llama-path feature (webgpu.js:1239-1270)")
         self.resetCache()
         t0 = time.perf_counter()
-        logits = self.forwardPrompt(ids)
+        logits = self.promptStep(ids) if mode == "sample" else self.forwardPrompt(ids)
         ttft = (time.perf_counter() - t0) * 1e3
         out: List[int] = []
         if mode == "sample":
