@@ -202,7 +202,10 @@ export class HipPetitGPT {
    * (device-chained, webgpu.js:1202-1226), "spec" (prompt-lookup speculation,
    * webgpu.js:1239-1270; llama models) or "sample" (draw() with the options
    * temperature, topK, topP, minP and random, a function of numbers of [0, 1),
-   * Math.random if it is not given).
+   * Math.random if it is not given; greedy at a temperature of 0).  GPT-2's
+   * 3-gram block and penalty (infer.js:252-287) belong to the greedy choice:
+   * they act at temperature 0, and above it tokens are drawn from the logits as
+   * they are.
    */
   async generate(inIds, opts) {
     const o = opts || {};
@@ -220,12 +223,14 @@ export class HipPetitGPT {
     if (mode === "spec" && this.isGpt2) throw new Error("speculative decode needs a llama-style model");
     this.resetCache();
     const t0 = now();
-    const logits = mode === "sample" ? this.promptStep(ids) : this.forwardPrompt(ids);
+    // GPT-2's greedy rule reads the logits on the host
+    const drawn = mode === "sample" && (!this.isGpt2 || o.temperature === undefined || o.temperature > 0);
+    const logits = drawn ? this.promptStep(ids) : this.forwardPrompt(ids);
     const ttft = now() - t0;
     const out = [];
     const random = o.random || Math.random;
     let next;
-    if (mode === "sample") next = this.draw(random(), o).id;
+    if (drawn) next = this.draw(random(), o).id;
     else next = this.isGpt2 ? argmaxGpt2(logits, []) : this.lastArgmax;
     out.push(next);
     let specHits = 0;
@@ -234,7 +239,7 @@ export class HipPetitGPT {
     if (onToken) await onToken(next, { phase: "prefill", ms: ttft });
     if (next === eosId) {
       stopReason = "eos";
-    } else if (mode === "greedy") {
+    } else if (mode === "greedy" || (mode === "sample" && !drawn)) {
       for (let i = 1; i < maxNewTokens; i++) {
         if (ids.length + out.length >= this.cfg.maxSeqLen) break;
         const step = this.forwardDecode(next);

@@ -13,7 +13,11 @@ generate() implements four drivers of the same decode step:
                  (webgpu.js:846-865) and verify k+1 positions in one pass,
                  greedy acceptance (webgpu.js:1239-1270)
   mode="sample"  host loop of forwardDecode + draw: temperature, top-k, top-p
-                 and min-p on the device (no reference counterpart)
+                 and min-p on the device (no reference counterpart); greedy at
+                 a temperature of 0.  GPT-2's 3-gram block and penalty
+                 (infer.js:252-287) belong to the greedy choice: they act at
+                 temperature 0, and above it tokens are drawn from the logits
+                 as they are
 """
 from __future__ import annotations
 
@@ -266,10 +270,12 @@ class PetitGPT:
             raise ValueError("speculative decode is a llama-path feature (webgpu.js:1239-1270)")
         self.resetCache()
         t0 = time.perf_counter()
-        logits = self.promptStep(ids) if mode == "sample" else self.forwardPrompt(ids)
+        # GPT-2's greedy rule reads the logits on the host
+        drawn = mode == "sample" and (temperature > 0 or not self.is_gpt2)
+        logits = self.promptStep(ids) if drawn else self.forwardPrompt(ids)
         ttft = (time.perf_counter() - t0) * 1e3
         out: List[int] = []
-        if mode == "sample":
+        if drawn:
             random = random or np.random.default_rng().random
             settings = dict(temperature=temperature, topK=topK, topP=topP, minP=minP)
             nxt = self.draw(random(), **settings)[0]
@@ -282,7 +288,7 @@ class PetitGPT:
             onToken(nxt, {"phase": "prefill", "ms": ttft})
         if nxt == eosId:
             stop = "eos"
-        elif mode == "greedy":
+        elif mode == "greedy" or (mode == "sample" and not drawn):
             for _ in range(1, maxNewTokens):
                 if len(ids) + len(out) >= c.max_seq_len:
                     break

@@ -46,3 +46,50 @@ def test_node_sampling_leaves_the_logits_on_the_device(tmp_path):
     (tmp_path / "spec.json").write_text(json.dumps(spec))
     out = run_node("run_sample_modes.mjs", str(tmp_path / "m.pgw"), str(tmp_path / "spec.json"))
     assert out["kept"] and out["drawn"] == out["greedy"]
+
+
+def repeating(kind):
+    """A GPT-2 whose plain argmax repeats itself, so that the 3-gram block acts."""
+    return pgw.make_model(pgw.small_config("gpt2"), seed=5, kind=kind)
+
+
+@gpu
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan")])
+@pytest.mark.parametrize("kind", ["q4", "f32"])
+def test_gpt2_at_temperature_0_is_greedy(kind, temperature):
+    import mllm
+
+    g = mllm.PetitGPT(pgw.parse_pgw(repeating(kind)))
+    prompt = [3, 14, 15, 92, 65]
+    greedy = g.generate(prompt, maxNewTokens=24)
+    got = g.generate(prompt, maxNewTokens=24, mode="sample", temperature=temperature, random=lambda: 0.5)
+    assert got["generatedIds"] == greedy["generatedIds"] and got["mode"].endswith("sample")
+    eos = greedy["generatedIds"][5]
+    stopped = g.generate(prompt, maxNewTokens=24, mode="sample", temperature=temperature, eosId=eos)
+    assert stopped["stopReason"] == "eos" and stopped["generatedIds"] == greedy["generatedIds"][:stopped_at(greedy, eos)]
+    # the rule has something to do: the maxima alone are other tokens
+    lg, plain = g.forwardPrompt(prompt), []
+    for _ in range(24):
+        plain.append(int(np.argmax(lg)))
+        lg = g.forwardDecode(plain[-1])
+    assert plain != greedy["generatedIds"]
+    g.destroy()
+
+
+def stopped_at(res, eos):
+    return res["generatedIds"].index(eos) + 1
+
+
+@gpu
+@pytest.mark.skipif(NODE is None, reason="node not installed")
+def test_node_gpt2_at_temperature_0_is_greedy(tmp_path):
+    import mllm
+
+    b = repeating("q4")
+    (tmp_path / "m.pgw").write_bytes(b)
+    spec = {"prompt": [3, 14, 15, 92, 65], "maxNewTokens": 24, "temperature": 0.0, "numbers": [0.5] * 24}
+    (tmp_path / "spec.json").write_text(json.dumps(spec))
+    out = run_node("run_sample_modes.mjs", str(tmp_path / "m.pgw"), str(tmp_path / "spec.json"))
+    g = mllm.PetitGPT(pgw.parse_pgw(b))
+    assert out["drawn"] == out["greedy"] == g.generate(spec["prompt"], maxNewTokens=24)["generatedIds"]
+    g.destroy()
