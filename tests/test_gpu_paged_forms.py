@@ -52,3 +52,197 @@ def test_padding_rows_hold_anything(rows, filler):
             assert not torch.equal(new[page, :, slot], old[page, :, slot])
             new[page, :, slot] = old[page, :, slot]
     assert torch.equal(pool.k, k0) and torch.equal(pool.v, v0)
+
+
+# ---------------------------------------------------------------- the plan's forms
+SIZE = {"f32": 4, "f16": 2, "bf16": 2}
+STORAGES = ["f32", "f16", "bf16"]
+MALL = 256 << 20   # more cache than this is read past the caches
+SHORT = 128 << 10  # a wave to a unit: rows of at most this many bytes a head ...
+MANY = 512         # ... and more units than this
+
+
+def most_heads(storage, hd):
+    """Query heads of a workgroup at most: 16, or 8 where a lane has more than
+    8 elements of a value."""
+    es, lanes = SIZE[storage], 4
+    while lanes * 16 < hd * es:
+        lanes *= 2
+    while lanes > 64 or hd % lanes or hd // lanes * es % 4:
+        lanes //= 2
+    return 16 if hd // lanes <= 8 else 8
+
+
+def parts_of(pool, rows, heads, max_len):
+    """The parts that the library's plan takes, from the workspace it asks for."""
+    kv, at = pool.desc(), p(pool.k)
+    rc = abi.lib().mllm_attn_paged(kv, rows, heads, at, at, at, max_len, 1.0, None, at, 0, None)  # refused: no out
+    msg = abi.lib().mllm_last_error().decode()
+    assert rc == 1
+    if "needed" not in msg:
+        assert "null pointer" in msg
+        return 1
+    rep, most = heads // pool.kv_heads, most_heads(pool.storage, pool.hd)
+    part = (min(rep, most) * (pool.hd + 2) + 3) // 4 * 4 * 4
+    units = rows * pool.kv_heads * -(-rep // most)
+    parts, rest = divmod(int(msg.split(" bytes, ")[1].split()[0]) - 16384, units * part)
+    assert rest == 0
+    return parts
+
+
+def holds(pool, q, seq, lens, heads, scale, max_len, some=None):
+    o = run_attn(pool, q, seq, lens, heads, scale, max_len=max_len)
+    some = list(range(len(lens))) if some is None else some
+    seqs = range(len(lens)) if seq is None else seq
+    ref, tol = ref_attn(q[some], pool, [seqs[r] for r in some], [lens[r] for r in some], heads, scale)
+    assert (np.abs(o[some] - ref) <= tol).all(), float((np.abs(o[some] - ref) / np.maximum(tol, 1e-38)).max())
+
+
+class LargePool(Pool):
+    """A pool past the Infinity Cache's size, made on the device; the sequences'
+    pages are drawn from all of it."""
+
+    def __init__(self, hd, storage, page, seqs, cols, seed):
+        self.page, self.hd, self.kv_heads, self.storage, self.strides = page, hd, 1, storage, (0, 0, 0)
+        es = SIZE[storage]
+        self.n = MALL // (2 * hd * es * page) + 9
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[storage]
+        self.k, self.v = (torch.empty(self.n, 1, page, hd, dtype=dt, device="cuda").normal_(generator=g) for _ in range(2))
+        self.table = torch.randint(0, self.n, (seqs, cols), generator=g, device="cuda").to(torch.int32)
+        self.kh, self.vh = self.k, self.v
+
+
+def head_counts(storage, hd):
+    """For the kernels of up to 4, 8 and (where there is one) 16 heads."""
+    return [3, 7] + ([13] if most_heads(storage, hd) > 8 else [])
+
+
+HDS = [32, 64, 96, 128, 160, 192, 224, 256]
+
+
+@gpu
+@pytest.mark.parametrize("hd", HDS)
+@pytest.mark.parametrize("storage", STORAGES)
+def test_attn_every_kernel_in_parts(storage, hd):
+    """Rows in several parts, joined: lengths in the first part, at its end and in all of them."""
+    g = torch.Generator().manual_seed(hd)
+    rng = np.random.default_rng(hd)
+    pool = Pool(g, 1, hd, 16, 5, 57, storage)
+    lens = [900, 1, 0, 128, 611]
+    for heads in head_counts(storage, hd) + [most_heads(storage, hd) + 2]:
+        assert parts_of(pool, 5, heads, 900) > 1
+        print(f"parts {storage} {hd} heads={heads}", flush=True)
+        holds(pool, rng.standard_normal((5, heads, hd)).astype(np.float32), None, lens, heads, 1 / math.sqrt(hd), 900)
+
+
+@gpu
+@pytest.mark.parametrize("hd", HDS)
+@pytest.mark.parametrize("storage", STORAGES)
+def test_attn_every_kernel_of_one_wave(storage, hd):
+    g = torch.Generator().manual_seed(hd + 1)
+    rng = np.random.default_rng(hd + 1)
+    top = min(150, SHORT // (2 * hd * SIZE[storage]))
+    rows, seqs = MANY + 9, 24
+    pool = Pool(g, 1, hd, 16, seqs, -(-top // 16), storage)
+    seq = [int(v) for v in rng.integers(0, seqs, rows)]
+    lens = [int(v) for v in rng.integers(0, top + 1, rows)]
+    lens[:4] = [top, 0, 1, top - 1]
+    for heads in head_counts(storage, hd):
+        assert parts_of(pool, rows, heads, top) == 1
+        print(f"one wave {storage} {hd} heads={heads}", flush=True)
+        holds(pool, rng.standard_normal((rows, heads, hd)).astype(np.float32), seq, lens, heads, 1 / math.sqrt(hd), top,
+              some=list(range(8)) + [rows // 2, rows - 1])
+
+
+@gpu
+@pytest.mark.parametrize("hd", HDS)
+@pytest.mark.parametrize("storage", STORAGES)
+def test_attn_every_kernel_past_the_caches(storage, hd):
+    """More cache than the Infinity Cache holds, in long parts: a row of two
+    parts and a bit, a short one, an empty one."""
+    page = 128
+    max_len = MALL // (3 * 2 * hd * SIZE[storage]) + 999
+    pool = LargePool(hd, storage, page, 3, -(-max_len // page), hd)
+    rng = np.random.default_rng(hd + 2)
+    assert min(3 * max_len, pool.n * page) * 2 * hd * SIZE[storage] > MALL
+    for heads in head_counts(storage, hd):
+        parts = parts_of(pool, 3, heads, max_len)
+        assert parts > 1
+        lens = [2 * (max_len // parts) + 300, 70, 0]
+        print(f"stream {storage} {hd} heads={heads} parts={parts} lens={lens}", flush=True)
+        holds(pool, rng.standard_normal((3, heads, hd)).astype(np.float32), None, lens, heads, 1 / math.sqrt(hd), max_len)
+
+
+@gpu
+@pytest.mark.parametrize("storage,hd,heads,cols", [
+    ("f16", 64, 3, 940), ("f32", 64, 3, 940), ("bf16", 128, 4, 940), ("f32", 128, 7, 700), ("f16", 64, 16, 940),
+    ("bf16", 64, 13, 940), ("f16", 256, 8, 400)])
+def test_attn_joins_of_more_than_64_parts(storage, hd, heads, cols):
+    """A join takes its parts 64 at a time: all of them there, 65 and fewer."""
+    g = torch.Generator().manual_seed(51)
+    rng = np.random.default_rng(51)
+    pool = Pool(g, 1, hd, 64, 1, cols, storage)
+    top = cols * 64
+    parts = parts_of(pool, 1, heads, top)
+    assert parts > 64
+    chunk = -(-top // parts)  # about: whole 128s
+    for n in (top, top - 1, 65 * chunk + 7, 5 * chunk, 1):
+        holds(pool, rng.standard_normal((1, heads, hd)).astype(np.float32), None, [n], heads, 1 / math.sqrt(hd), top)
+
+
+@gpu
+@pytest.mark.parametrize("storage,hd,heads", [("f16", 32, 8), ("f32", 32, 20), ("bf16", 32, 36), ("f16", 64, 32), ("f32", 64, 8)])
+def test_attn_parts_of_more_than_2048_positions(storage, hd, heads):
+    """A workgroup of four waves looks up 2048 places at a time."""
+    g = torch.Generator().manual_seed(52)
+    rng = np.random.default_rng(52)
+    pool = Pool(g, 4, hd, 24, 6, 210, storage)
+    rows, top = 64, 5000
+    lens = [0, 1, 2047, 2048, 2049, 2200, 4095, 4096, 4097, 5000] + [int(v) for v in rng.integers(0, top + 1, rows - 10)]
+    seq = [int(v) for v in rng.integers(0, 6, rows)]
+    assert top // parts_of(pool, rows, heads, top) > 2048
+    q = rng.standard_normal((rows, heads, hd)).astype(np.float32)
+    holds(pool, q, seq, lens, heads, 1 / math.sqrt(hd), top, some=list(range(14)))
+
+
+@gpu
+@pytest.mark.parametrize("storage,heads,kvh,hd", [("f32", 9, 3, 64), ("f32", 4, 1, 128), ("f32", 15, 5, 64), ("bf16", 9, 3, 64)])
+@pytest.mark.parametrize("lens", [[700], [3000], [257, 1500, 700]])
+def test_attn_rows_of_a_chat_in_parts(storage, heads, kvh, hd, lens):
+    """The engine's default storage and shapes at a chat's lengths."""
+    g = torch.Generator().manual_seed(53)
+    rng = np.random.default_rng(53)
+    pool = Pool(g, kvh, hd, 16, len(lens), -(-max(lens) // 16), storage)
+    assert parts_of(pool, len(lens), heads, max(lens)) > 1
+    holds(pool, rng.standard_normal((len(lens), heads, hd)).astype(np.float32), None, lens, heads, 1 / math.sqrt(hd), max(lens))
+
+
+@gpu
+@pytest.mark.parametrize("top", [512, 700])
+def test_attn_rows_that_fill_the_chip_are_not_split(top):
+    """300 rows of 4 KV heads run in one part, without a workspace; one of them
+    alone is split, and refused without one."""
+    g = torch.Generator().manual_seed(54)
+    rng = np.random.default_rng(54)
+    rows, heads, alone = 300, 8, 900
+    pool = Pool(g, 4, 64, 16, 20, -(-alone // 16), "f16")
+    seq = [r % 20 for r in range(rows)]
+    lens = [int(v) for v in rng.integers(0, top + 1, rows)]
+    lens[0], lens[7] = top, top - 3
+    q = rng.standard_normal((rows, heads, 64)).astype(np.float32)
+    dev = lambda a, t: torch.tensor(np.asarray(a), dtype=t, device="cuda")  # noqa: E731
+    dq, ds, dl = dev(q.reshape(rows, -1), torch.float32), dev(seq, torch.int32), dev(lens, torch.int32)
+    out, kv = torch.full((rows, heads * 64), 7.0, device="cuda"), pool.desc()
+    abi.call("mllm_attn_paged", kv, rows, heads, p(dq), p(ds), p(dl), top, 0.125, p(out), None, 0, None)
+    torch.cuda.synchronize()
+    o = out.cpu().numpy().reshape(rows, heads, 64)
+    some = [0, 7, 8, 150, 299]
+    ref, tol = ref_attn(q[some], pool, [seq[r] for r in some], [lens[r] for r in some], heads, 0.125)
+    assert (np.abs(o[some] - ref) <= tol).all()
+    assert parts_of(pool, 1, heads, alone) > 1
+    for i, r in enumerate(some[:2]):
+        assert abi.lib().mllm_attn_paged(kv, 1, heads, p(dq), p(ds), p(dl), alone, 0.125, p(out), None, 0, None) == 1
+        assert b"needed" in abi.lib().mllm_last_error()
+        one = run_attn(pool, q[r:r + 1], [seq[r]], [lens[r]], heads, 0.125, max_len=alone)
+        assert (np.abs(one[0] - ref[i]) <= tol[i]).all()
