@@ -191,6 +191,10 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  *     out[r] (the heads' rows) is NaN.
  *   - Only positions below len[r] count, whatever the slots behind them hold.
  *     Infinities and NaN within it act as in infer.js:461-504.
+ *   - The values are summed under weights of up to e^8 and divided by the
+ *     weights' sum at the end: finite values stay finite where the largest
+ *     magnitude times len[r] is at most 2^116 (8.3e34).  Beyond that a sum may
+ *     pass float32's range: infinity or NaN.
  * Sums and the products with the values are float32; the queries multiply the
  * keys as float32 too, with an f16 cache as two f16 pieces (22 bits).  The
  * workspace is mllm_attn_paged_workspace() bytes, 16-byte aligned (NULL where

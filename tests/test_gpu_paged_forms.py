@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 from mllm import abi
-from test_gpu_paged import Pool, p, ref_attn, ref_rope, run_attn, run_rope
+from test_gpu_paged import TYPES, Pool, p, ref_attn, ref_rope, run_attn, run_rope
 
 torch = pytest.importorskip("torch")
 gpu = pytest.mark.gpu
@@ -246,3 +246,30 @@ def test_attn_rows_that_fill_the_chip_are_not_split(top):
         assert b"needed" in abi.lib().mllm_last_error()
         one = run_attn(pool, q[r:r + 1], [seq[r]], [lens[r]], heads, 0.125, max_len=alone)
         assert (np.abs(one[0] - ref[i]) <= tol[i]).all()
+
+
+@gpu
+@pytest.mark.parametrize("storage,hd", [("f32", 64), ("bf16", 128), ("f32", 256)])
+@pytest.mark.parametrize("rows,n", [(1, 700), (1, 64), (600, 64), (150, 700)])
+def test_attn_values_at_the_documented_bound(storage, hd, rows, n):
+    """Values of 2^116 / length, of one sign in an element, under weights of
+    nearly e^8: each wave's first 16 positions score 0, the others 255 / 32.
+    The sums come to 2^127.4 and stay finite."""
+    g = torch.Generator().manual_seed(61)
+    rng = np.random.default_rng(61)
+    pool = Pool(g, 4, hd, 16, 1, -(-n // 16), storage)
+    many = rows > 100
+    assert many or n == 64 or parts_of(pool, rows, 4, n) > 1
+    big = math.floor(2.0 ** 116 / n / 2.0 ** 100) * 2.0 ** 100
+    big = float(int(big / 2.0 ** (math.frexp(big)[1] - 8))) * 2.0 ** (math.frexp(big)[1] - 8)  # eight bits, for bf16
+    v = torch.from_numpy(rng.choice([-big, big], (4, n, hd)))
+    v[:, :, 0], v[:, :, 1] = big, -big
+    pool.kh.zero_()
+    for i in range(n):
+        page, slot = int(pool.table[0, i // 16]), i % 16
+        pool.kh[page, :, slot, 0] = 0.0 if (i if many else i % 128) < 64 and n > 64 or i < 16 else 255 / 32
+        pool.vh[page, :, slot] = v[:, i].to(TYPES[storage]).cuda()
+    q = np.zeros((rows, 4, hd), np.float32)
+    q[:, :, 0] = 8.0
+    some = [0, rows - 1]
+    holds(pool, q, [0] * rows, [n] * rows, 4, 0.125, n, some=some)
