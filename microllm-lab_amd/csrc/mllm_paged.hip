@@ -34,10 +34,14 @@ struct RopeArgs {
 // of 128 (360 MB), us: runs of eight elements a lane, which touch every cache
 // line twice, 124; runs of four 75, three heads of a lane in flight 88, three
 // times the threads 98; loads and stores past the caches, whose readers sit
-// behind another L2, 70 (5.2 TB/s; a large copy moves 4.8).
+// behind another L2, 70 (5.2 TB/s; a copy of the same bytes takes 72).  Element
+// by element, 60 of the 128 rotated: 222.
 //
 // The angle is formed in double and in turns: a position of 2^20 keeps 2^-33
-// of a turn, where a float product would keep 2^-4.
+// of a turn, where a float product would keep 2^-4.  What is left of it within
+// half a turn is rounded to float for the sine and cosine: they are off by at
+// most pi 2^-25 (9.4e-8) for it, as much as their own rounding costs, which
+// keeps the double functions out of every lane.
 template <class KV, bool VEC>
 __global__ __launch_bounds__(WG) void k_rope_kv(RopeArgs A) {
   const int token = blockIdx.x, lph = 1 << A.lg_lph, s = threadIdx.x & (lph - 1);
@@ -183,9 +187,9 @@ hipStream_t as_stream(void *s) { return reinterpret_cast<hipStream_t>(s); }
 constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
 
 // Positions per workgroup (turns of the four waves) and the number of parts for
-// rows of up to max_len positions.  A CU reads at most about 28 GB/s, whatever
-// the number of its workgroups, and the chip 6.2 TB/s: the time goes by the
-// bytes of the CU that has most, a workgroup's start and end (about 64 KB of
+// rows of up to max_len positions.  With this kernel's loads a CU comes to about
+// 28 GB/s, with one workgroup or more, and the chip to 6.2 TB/s: the time goes by
+// the bytes of the CU that has most, a workgroup's start and end (about 64 KB of
 // reading) and a join (96 KB).  Measured, us: 2 rows of 100000 positions, 16
 // units, 8 / 12 / 16 / 20 / 24 / 32 parts 239 / 174 / 143 / 199 / 168 / 152; 320
 // units of 6144 positions, 1 / 2 / 3 / 4 / 6 parts 111 / 98 / 89 / 88 / 99; 100
@@ -195,14 +199,16 @@ constexpr int64_t kMallBytes = 256 << 20;  // the Infinity Cache
 // 516 in f16 9.7 / 9.1 / 9.2.
 // At most kCounters workgroups where rows are split: a workspace for many rows
 // and long ones serves fewer and shorter.
-// Many short rows (more units than the two workgroups of four waves that a CU
-// holds, of at most kShort bytes each) take a wave to a unit, so that eight of
-// them are at their starts and ends at once.  Four waves / one, us: 640 units of
-// 64 f16 elements, 16 / 128 / 512 / 1024 positions 10.6 / 9.0, 12.0 / 9.1, 20.2
-// / 17.6, 36.1 / 35.3; 320 units 8.7 / 8.7, 8.8 / 8.7, 13.4 / 16.6, 20.3 / 28.3;
-// 2560 units 28.6 / 11.7, 32.9 / 19.3, 65.8 / 66.5, 110 / 126; 2048 units of 128
-// bf16 elements, 25 / 128 / 256 / 512 positions 24.7 / 11.7, 35.5 / 25.5, 61.4
-// / 52.2, 91.0 / 95.4.
+// Many short rows (more than two units to a CU, of at most kShort bytes each)
+// take a wave to a unit, so that eight of them are at their starts and ends at
+// once.  Two is what a CU holds of the workgroups of four waves measured here;
+// by its registers a form has one to four (f32 heads of 64 four, f32 and bf16
+// heads of 256 with more than four query heads one), where it was not measured.
+// Four waves / one, us: 640 units of 64 f16 elements, 16 / 128 / 512 / 1024
+// positions 10.6 / 9.0, 12.0 / 9.1, 20.2 / 17.6, 36.1 / 35.3; 320 units 8.7 /
+// 8.7, 8.8 / 8.7, 13.4 / 16.6, 20.3 / 28.3; 2560 units 28.6 / 11.7, 32.9 / 19.3,
+// 65.8 / 66.5, 110 / 126; 2048 units of 128 bf16 elements, 25 / 128 / 256 / 512
+// positions 24.7 / 11.7, 35.5 / 25.5, 61.4 / 52.2, 91.0 / 95.4.
 constexpr int64_t kShort = 128 << 10;
 constexpr int64_t kChunk = 128, kCus = 256, kStart = 64 << 10, kJoinCost = 96 << 10;
 void attn_plan(int64_t units, int max_len, int64_t pos_bytes, int *waves, int *chunk, int *splits) {

@@ -38,11 +38,12 @@ namespace {
 // What bounds it: a row's own chain, since a row has one CU.  Of 49152 logits,
 // us: the maxima 4.5 (44 GB/s), the histogram of all weights 14.7 (each wave
 // issues about 1000 instructions, 6.7 on the four SIMDs, the rest is the
-// atomics), the list 5, a draw from a short list 5.  Measured: one row with
-// top-k and top-p 14.1, 100 rows of 131072 with min-p 24.7 (2.1 TB/s), 200 rows of
-// 49152 with top-p alone 60, 64 rows of 50257 with every setting 54 -- there the
-// rows whose top-p leaves more tokens than the list holds set the time: they
-// weigh all tokens twice.  Tried without gain: the row kept in registers between the
+// atomics), the list 5, a draw from a short list 5.  Measured, the mean of four
+// sets of inputs: one row with top-k and top-p 16, without a filter 24; 100 rows of
+// 131072 with min-p 26.5 (2.0 TB/s), 64 rows of 49152 without a filter 26, 200 rows
+// of 49152 with top-p alone 56, 64 rows of 50257 with every setting 50 -- there the
+// rows whose top-p leaves more tokens than the list holds set the time: they weigh
+// all tokens twice.  Tried without gain: the row kept in registers between the
 // passes (it spills), more waves (there are none).
 constexpr int ST = 1024;        // threads
 constexpr int SW = ST / 64;     // waves
