@@ -39,9 +39,8 @@ struct RopeArgs {
 //
 // The angle is formed in double and in turns: a position of 2^20 keeps 2^-33
 // of a turn, where a float product would keep 2^-4.  What is left of it within
-// half a turn is rounded to float for the sine and cosine: they are off by at
-// most pi 2^-25 (9.4e-8) for it, as much as their own rounding costs, which
-// keeps the double functions out of every lane.
+// half a turn is taken as two floats, hi + lo: the functions of hi, and their
+// slopes times lo (at most 2^-25 of half a turn; its square is below 2^-47).
 template <class KV, bool VEC>
 __global__ __launch_bounds__(WG) void k_rope_kv(RopeArgs A) {
   const int token = blockIdx.x, lph = 1 << A.lg_lph, s = threadIdx.x & (lph - 1);
@@ -101,7 +100,11 @@ __global__ __launch_bounds__(WG) void k_rope_kv(RopeArgs A) {
     sn[j] = 0.f, cs[j] = 1.f;
     if (in && 2 * pair(j) < A.rot) {
       const double t = (double)pos * ((double)A.inv_freq[pair(j)] * 0.15915494309189533577);  // turns
-      sincospif((float)(2.0 * (t - rint(t))), &sn[j], &cs[j]);
+      const double x = 2.0 * (t - rint(t));
+      const float hi = (float)x, lo = (float)(x - (double)hi) * 3.14159265f;
+      float sh, ch;
+      sincospif(hi, &sh, &ch);
+      sn[j] = __builtin_fmaf(ch, lo, sh), cs[j] = __builtin_fmaf(-sh, lo, ch);
     }
   }
   auto store = [&](bool r, const float (&u)[4], const float (&w)[4], auto *to, auto put) {

@@ -273,3 +273,31 @@ def test_attn_values_at_the_documented_bound(storage, hd, rows, n):
     q[:, :, 0] = 8.0
     some = [0, rows - 1]
     holds(pool, q, [0] * rows, [n] * rows, 4, 0.125, n, some=some)
+
+
+@gpu
+@pytest.mark.parametrize("inter", [0, 1])
+def test_rope_angles_keep_double_precision(inter):
+    """Heads of (1, 0) in each pair are (cos, sin) after the rotation.  The angle
+    comes in double, so they are the float functions' values (1 step at most) and
+    one addition (half a step): 1.5 steps of the value.  For values near 0 there
+    are the part that two float parts of the angle leave, 2^-47, and the angle's
+    own roundings in double, half a step of it each: 1 / (2 pi), its product with
+    the frequency, that with the position, and the oracle's product."""
+    hd, T = 64, 4096
+    g = torch.Generator().manual_seed(71)
+    rng = np.random.default_rng(71)
+    pool = Pool(g, 1, hd, 1024, 1, 64, "f32")
+    pos = rng.permutation(65536)[:T].astype(np.int32)
+    freq = rng.uniform(0.0, 3.0, hd // 2).astype(np.float32)
+    x = np.zeros((T, 3, hd), np.float32)
+    i = np.arange(hd // 2)
+    a, b = (2 * i, 2 * i + 1) if inter else (i, i + hd // 2)
+    x[:, :, a] = 1.0
+    q = run_rope(pool, x.reshape(T, -1), np.zeros(T, np.int32), pos, freq, hd, inter, None, None, 1).cpu().numpy()
+    ang = pos.astype(np.float64)[:, None] * freq.astype(np.float64)
+    for got, want in ((q[:, a], np.cos(ang)), (q[:, b], np.sin(ang))):
+        err = np.abs(got - want)
+        step = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64)
+        tol = 1.5 * step + 2.0 ** -47 + 4 * 2.0 ** -53 * ang
+        assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
