@@ -301,3 +301,15 @@ def test_rope_angles_keep_double_precision(inter):
         step = np.spacing(np.abs(want).astype(np.float32)).astype(np.float64)
         tol = 1.5 * step + 2.0 ** -47 + 4 * 2.0 ** -53 * ang
         assert (err <= tol).all(), (float((err / tol).max()), float(err.max()))
+
+
+@gpu
+@pytest.mark.parametrize("rows", [3, 600])
+def test_attn_no_positions_at_all(rows):
+    """max_len 0: empty rows are 0, padding stays, any length is too long."""
+    g = torch.Generator().manual_seed(81)
+    pool = Pool(g, 2, 64, 16, 5, 1, "f16", fill=float("nan"))
+    seq, lens = [r % 5 for r in range(rows)], [0] * rows
+    seq[1], lens[2] = -1, 1
+    o = run_attn(pool, np.ones((rows, 4, 64), np.float32), seq, lens, 4, 0.125, max_len=0)
+    assert (o[1] == 7.0).all() and np.isnan(o[2]).all() and (np.delete(o, [1, 2], 0) == 0).all()
