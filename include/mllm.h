@@ -190,7 +190,8 @@ int mllm_rope_kv_paged(const mllm_kv_pages *kv, int tokens, int n_heads, const f
  *   - len[r] < 0 or > max_len, or a page within the length outside [0, pages):
  *     out[r] (the heads' rows) is NaN.
  *   - Only positions below len[r] count, whatever the slots behind them hold.
- *     Infinities and NaN within it act as in infer.js:461-504.
+ *     Infinities and NaN within it act as in infer.js:461-504; weights below
+ *     about 2^-126 of the largest count as 0 (times an infinite value: NaN).
  *   - The values are summed under weights of up to e^8 and divided by the
  *     weights' sum at the end: finite values stay finite where the largest
  *     magnitude times len[r] is at most 2^116 (8.3e34).  Beyond that a sum may
