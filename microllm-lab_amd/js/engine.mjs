@@ -224,7 +224,7 @@ export class HipPetitGPT {
     this.resetCache();
     const t0 = now();
     // GPT-2's greedy rule reads the logits on the host
-    const drawn = mode === "sample" && (!this.isGpt2 || o.temperature === undefined || o.temperature > 0);
+    const drawn = mode === "sample" && (!this.isGpt2 || o.temperature === undefined || Math.fround(o.temperature) > 0);
     const logits = drawn ? this.promptStep(ids) : this.forwardPrompt(ids);
     const ttft = now() - t0;
     const out = [];

@@ -271,7 +271,7 @@ class PetitGPT:
         self.resetCache()
         t0 = time.perf_counter()
         # GPT-2's greedy rule reads the logits on the host
-        drawn = mode == "sample" and (temperature > 0 or not self.is_gpt2)
+        drawn = mode == "sample" and (np.float32(temperature) > 0 or not self.is_gpt2)
         logits = self.promptStep(ids) if drawn else self.forwardPrompt(ids)
         ttft = (time.perf_counter() - t0) * 1e3
         out: List[int] = []

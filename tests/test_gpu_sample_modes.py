@@ -54,7 +54,7 @@ def repeating(kind):
 
 
 @gpu
-@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan")])
+@pytest.mark.parametrize("temperature", [0.0, -1.0, float("nan"), 1e-50])  # the last is 0 in float32
 @pytest.mark.parametrize("kind", ["q4", "f32"])
 def test_gpt2_at_temperature_0_is_greedy(kind, temperature):
     import mllm
