@@ -165,7 +165,8 @@ typedef struct mllm_kv_pages {
  *     pass through: pairs (i, i + rot / 2) (applyRope, infer.js:208-225), or
  *     (2i, 2i + 1) where interleaved != 0, by the angle pos * inv_freq[i],
  *     i < rot / 2, formed in double; its sine and cosine are float32.  A
- *     context scaled for more positions is a matter of inv_freq.  rot = 0 rotates nothing (inv_freq may be NULL).
+ *     context scaled for more positions is a matter of inv_freq.  rot = 0
+ *     rotates nothing (inv_freq may be NULL).
  *   - q (like qkv 16-byte aligned) receives [tokens][n_heads head_dim]; keys and values go to the token's
  *     slot, rounded to nearest even (f16: beyond 65504 to infinity).
  * A token whose sequence is outside [0, sequences), or whose position is

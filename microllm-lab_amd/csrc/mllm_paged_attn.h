@@ -159,9 +159,10 @@ __device__ __forceinline__ v4f mma32(u32x4 a, u32x4 b, v4f c) {
 // come to, not what a CU can read) and 6.2 to 6.4 TB/s in all, and for short rows a
 // workgroup's start and end.  Per 64 positions of an f16 head of 64 elements, 16
 // KB, a wave spends 16 + 64 MFMAs (770 cycles) and about 1000 VALU cycles; a
-// SIMD's share of the CU's 28 GB/s is 5600 cycles for them.  Measured, us: 2
-// rows of 100000 positions, 8 heads of 128 bf16 elements (819 MB), 143 (5.7 TB/s), of f16 143, of f32 (1638 MB) 255; 64 rows of 512 to
-// 2048, 5 heads of 64 f16 or bf16 elements (102 MB), 30.5, of f32 (203 MB) 45.8;
+// SIMD's share of the CU's 28 GB/s is 5600 cycles for them.  Measured, us: 2 rows
+// of 100000 positions, 8 heads of 128 bf16 or f16 elements (819 MB), 143 (5.7
+// TB/s), of f32 (1638 MB) 255; 64 rows of 512 to 2048, 5 heads of 64 f16 or bf16
+// elements (102 MB), 30.5, of f32 (203 MB) 45.8;
 // 2560 units of 128 positions, a wave to each (88 MB), 22; 64 rows, 8 query heads
 // to a KV head of 256, one workgroup to a CU: bf16 (177 MB) 48, f32 (349 MB) 76.
 // In the 102 MB of f16 a workgroup takes 1.0 to its row's length, 1.4 to its pages,
