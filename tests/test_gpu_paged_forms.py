@@ -313,3 +313,19 @@ def test_attn_no_positions_at_all(rows):
     seq[1], lens[2] = -1, 1
     o = run_attn(pool, np.ones((rows, 4, 64), np.float32), seq, lens, 4, 0.125, max_len=0)
     assert (o[1] == 7.0).all() and np.isnan(o[2]).all() and (np.delete(o, [1, 2], 0) == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("storage,low", [("f16", -20), ("f16", -15), ("bf16", -128)])
+@pytest.mark.parametrize("which", ["k", "v"])
+def test_attn_subnormal_keys_and_values(storage, low, which):
+    """Keys or values below the type's least normal number count for what they are."""
+    g = torch.Generator().manual_seed(91)
+    rng = np.random.default_rng(91)
+    pool = Pool(g, 2, 64, 16, 1, 20, storage)
+    t = pool.k if which == "k" else pool.v
+    t.copy_((t.double() * 2.0 ** low).to(t.dtype))
+    up = min(-low, 100) if which == "k" else 0
+    scale = 0.125 * 2.0 ** ((-low if which == "k" else 0) - up)
+    q = (rng.standard_normal((1, 6, 64)) * 2.0 ** up).astype(np.float32)
+    holds(pool, q, None, [310], 6, scale, 310)
